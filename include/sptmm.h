@@ -283,7 +283,7 @@ int sptmm_gemv_f32(const sptmm_weights *w, const float *X_dev, int M, float *C_d
  * in fp32 (evaluated in this order).  One launch where the unfused sequence takes
  * three (quantise, GEMV, rescale).  The reference has the GEMV only; it passes
  * an unused scale to its i2s kernel (main.cu:1862).  u16 and gap streams. */
-typedef enum sptmm_xtype { SPTMM_X_F16 = 1, SPTMM_X_BF16 = 2 } sptmm_xtype;
+typedef enum sptmm_xtype { SPTMM_X_F16 = 1, SPTMM_X_BF16 = 2, SPTMM_X_F32 = 3 /* rows of sptmm_heads_norm_rotate only */ } sptmm_xtype;
 int sptmm_gemv_q8(const sptmm_weights *w, const uint16_t *X_dev, int x_type, int M, float w_scale, float *Y_dev, void *stream);
 /* The rescale alone, for callers whose activations are int8 already (quantised by the operator in front, which also
  * left the rows' 1/s_m -- a_m / 127 -- in device memory): the sums of sptmm_gemv_i8 written as
@@ -321,6 +321,93 @@ int sptmm_gemv_i8_batched(const sptmm_weights *const *ws, const int8_t *const *X
  * (float out; u16 and gap streams only). */
 int sptmm_gemv_batched(const sptmm_weights *const *ws, const void *const *X_dev, void *const *C_dev, int count, int M,
                        int act, void *stream);
+
+/* ---------------------------------------------- between the projections of a decoder layer
+ * What stands between two GEMVs of a layer (no counterpart in the reference, which has the products only):
+ *   q+k+v projection -> adapters -> heads -> attention -> o projection -> adapters
+ * Rows are row-major device buffers as above; all calls are asynchronous on `stream`, allocate nothing, hold no state
+ * between calls, and may be captured into a graph.  Every buffer belongs to the current device.  What device arrays say
+ * (slots, positions, cache rows, lengths) is read by the kernels and cut to the sizes given here, so that no value in them
+ * leads out of a buffer. */
+
+/* Low-rank adapters of many requests beside one shared projection:
+ *     Y[m][n] = base[m][n] + scale_s * sum_r B_s[n][r] * (sum_k A_s[r][k] X[m][k]),   s = row_slot[m]
+ * A set holds `slots` adapters for one K x N projection, each of any rank up to max_rank (1..256), weights fp16 or bf16
+ * (sptmm_xtype).  Products of 16-bit values are summed in 32 bits, and the inner sums stay in 32 bits.
+ *   sptmm_adapters_set: copies A [rank][K] and B [N][rank] (dense row-major device buffers) into a slot, on `stream`; rank 0 empties it.
+ *     The caller orders it against sptmm_adapters_apply calls that use the slot on other streams.
+ *   sptmm_adapters_apply: X [M][K] of the set's type (what sptmm_gemv_q8 takes), base and Y [M][N] float (what it leaves).
+ *     base may be Y (added in place) or NULL (zeros).  row_slot[m] outside 0..slots-1, or an empty slot: Y[m] = base[m].
+ *     Rows of one slot need not lie together.  An Inf or NaN in one row or one adapter reaches the rows that use it only.
+ *     workspace_dev: sptmm_adapters_workspace_bytes(a, M) bytes, the caller's, reusable from call to call on one stream;
+ *     calls that may overlap need one each.  X, base, Y and the workspace are aligned to 16 bytes.
+ * A set is used with the device current on which it was made (SPTMM_ERR_INVALID otherwise). */
+typedef struct sptmm_adapters sptmm_adapters; /* opaque; owns its device buffers */
+int sptmm_adapters_create(int K, int N, int type, int slots, int max_rank, sptmm_adapters **out);
+int sptmm_adapters_set(sptmm_adapters *a, int slot, const uint16_t *A_dev, const uint16_t *B_dev, int rank, float scale, void *stream);
+size_t sptmm_adapters_workspace_bytes(const sptmm_adapters *a, int M);
+int sptmm_adapters_apply(const sptmm_adapters *a, const uint16_t *X_dev, const int32_t *row_slot_dev, int M, const float *base_dev, float *Y_dev,
+                         void *workspace_dev, size_t workspace_bytes, void *stream);
+void sptmm_adapters_free(sptmm_adapters *a);
+
+/* Angles of a rotation by position: pair j of a head turns by position * radians_per_position[j] (for the usual geometric
+ * sequence base^(-2j / rotated)).  interleaved 0: pair j is elements j and j + pairs; 1: elements 2j and 2j + 1.  Elements from
+ * 2 * pairs on are not turned.  The frequencies are kept as 64-bit fractions of a turn, so the phase of any 32-bit
+ * position is exact to 2^-33 of a turn.  Plain data: copy it, keep it on the stack. */
+#define SPTMM_MAX_ROTATED_PAIRS 128
+typedef struct sptmm_rotation {
+    int pairs;
+    int interleaved;
+    uint64_t turns[SPTMM_MAX_ROTATED_PAIRS];
+} sptmm_rotation;
+int sptmm_rotation_init(const double *radians_per_position, int pairs, int interleaved, sptmm_rotation *out);
+
+/* Query, key and value heads from the projection's rows, in one pass: RMS norm of every query and key head over its
+ * head_dim elements (x * rsqrt(mean(x^2) + eps) * gain), rotation by position, rounding to 16 bits, keys and values to their cache rows.
+ * Everything in 32 bits, rounded once.  Heads of a row lie head_dim apart; strides are in elements. */
+typedef struct sptmm_heads_args {
+    const void *q, *k, *v;                 /* rows of q_heads / kv_heads / kv_heads heads (parts of one fused row, or separate); v may be NULL: no values */
+    int64_t q_stride, k_stride, v_stride;
+    int in_type;                           /* SPTMM_X_F32, SPTMM_X_F16 or SPTMM_X_BF16 */
+    int out_type;                          /* SPTMM_X_F16 or SPTMM_X_BF16 */
+    void *q_out, *k_out, *v_out;           /* q_out: row t; k_out and v_out: row kv_rows[t], or t.  Either input buffer may be its own output
+                                            * (16-bit rows of the same type and stride, kv_rows NULL); no other overlap */
+    int64_t q_out_stride, k_out_stride, v_out_stride;
+    int tokens, q_heads, kv_heads, head_dim; /* head_dim even, 2..256; either head count may be 0 */
+    const int32_t *positions;              /* [tokens]; NULL: 0, 1, 2, ... */
+    const int32_t *kv_rows;                /* [tokens] distinct rows of k_out / v_out, or NULL: row t; a row outside 0..kv_capacity-1 is not stored */
+    int64_t kv_capacity;                   /* rows of k_out and v_out */
+    const float *q_gain, *k_gain;          /* [head_dim] each; NULL: these heads are not normalised */
+    float eps;
+    const sptmm_rotation *rotation;        /* host memory, read by the call; NULL: no rotation */
+} sptmm_heads_args;
+int sptmm_heads_norm_rotate(const sptmm_heads_args *args, void *stream);
+
+/* Causal attention with grouped heads over packed sequences.  Sequence b has the query rows q_start[b] .. q_start[b+1]-1 of q
+ * and the keys and values kv_start[b] .. kv_start[b]+kv_len[b]-1 of the cache; its query i of n sees keys j <= kv_len[b] - n + i
+ * (whole prompts: n = kv_len; one token against a cache: n = 1; chunks of prompts in between; rows that see nothing become
+ * zeros).  kv_start and kv_len NULL: the keys are packed as the queries are.  Query head h reads key/value head
+ * h / (q_heads / kv_heads).  16-bit inputs and outputs; products summed, and softmax statistics kept, in 32 bits.
+ * Output row i depends on the keys and values it sees only: Inf or NaN in other rows of the cache do not reach it.  Rows of
+ * `out` behind the last sequence are left as they were.
+ * max_q and max_kv (host side: at least the longest sequence's queries and keys) choose how the work is cut up; the results
+ * are right whatever they say.
+ * workspace_dev: sptmm_attention_workspace_bytes(args) bytes (0: may be NULL), aligned to 16, the caller's, reusable from
+ * call to call on one stream; calls that may overlap need one each. */
+typedef struct sptmm_attention_args {
+    const uint16_t *q, *k, *v;
+    uint16_t *out;
+    int64_t q_stride, k_stride, v_stride, out_stride; /* elements between rows: multiples of 8 (out: of 4); k and v at most 2^22 */
+    int64_t kv_rows;                                  /* rows of k and v, at most 2^30 */
+    const int32_t *q_start;                           /* [batch + 1], not decreasing, q_start[batch] <= total_q */
+    const int32_t *kv_start, *kv_len;                 /* [batch] each, or both NULL */
+    int batch, total_q, max_q, max_kv;
+    int q_heads, kv_heads, head_dim;                  /* head_dim a multiple of 8, 8..256 */
+    int type;                                         /* SPTMM_X_F16 or SPTMM_X_BF16 */
+    float scale;                                      /* of the scores, positive */
+} sptmm_attention_args;
+size_t sptmm_attention_workspace_bytes(const sptmm_attention_args *args);
+int sptmm_attention(const sptmm_attention_args *args, void *workspace_dev, size_t workspace_bytes, void *stream);
 
 /* Thin device-memory / stream / event helpers so callers need no HIP headers
  * (the cudaMalloc/cudaMemcpy/cudaEvent* calls of main.cu:767-782, 804-815). */

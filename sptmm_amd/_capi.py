@@ -11,10 +11,12 @@ __all__ = [
     "pack_u16", "unpack_u16", "delta_bits", "pack_delta", "unpack_delta", "pack_i2s", "unpack_i2s", "pack_ragged", "unpack_ragged",
     "generate_ternary_iid", "dense_from_i2s_words", "choose_split_k", "wide_k_tile", "pack_wide", "unpack_wide",
     "i2s_pack_word", "i2s_decode_word", "Weights", "DeviceBuffer", "Stream", "Event", "copy_kernel", "read_kernel",
-    "device_sync", "Graph", "measure_gemv", "measure_sequence", "Step", "SEQ_MODES", "PlanStruct", "gemv_i8_batched", "gemv_batched", "KIND_U16", "KIND_DELTA", "KIND_I2S", "EXPORTS",
+    "device_sync", "Graph", "measure_gemv", "measure_sequence", "Step", "SEQ_MODES", "PlanStruct", "gemv_i8_batched", "gemv_batched", "KIND_U16", "KIND_DELTA", "KIND_I2S",
+    "X_F16", "X_BF16", "X_F32", "Adapters", "Rotation", "HeadsArgs", "heads_norm_rotate", "AttentionArgs", "attention", "attention_workspace_bytes", "EXPORTS",
 ]
 
 KIND_U16, KIND_DELTA, KIND_I2S = 1, 2, 3
+X_F16, X_BF16, X_F32 = 1, 2, 3
 # modes of sptmm_measure_sequence
 SEQ_MODES = {"launches": 0, "graph_chain": 1, "graph_branches": 2, "streams": 3, "batched_pairs": 4}
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -39,6 +41,8 @@ EXPORTS = [
     "sptmm_event_elapsed_us", "sptmm_measure_gemv", "sptmm_copy_kernel", "sptmm_read_kernel",
     "sptmm_graph_begin", "sptmm_graph_end", "sptmm_graph_launch", "sptmm_graph_destroy",
     "sptmm_stream_wait_event", "sptmm_measure_sequence", "sptmm_weights_set_plan", "sptmm_weights_get_plan", "sptmm_weights_tune",
+    "sptmm_adapters_create", "sptmm_adapters_set", "sptmm_adapters_workspace_bytes", "sptmm_adapters_apply", "sptmm_adapters_free",
+    "sptmm_rotation_init", "sptmm_heads_norm_rotate", "sptmm_attention_workspace_bytes", "sptmm_attention",
 ]
 
 
@@ -70,6 +74,66 @@ class PlanStruct(C.Structure):
 class Step(C.Structure):
     """sptmm_step: one GEMV of a sequence (see sptmm_measure_sequence)."""
     _fields_ = [("w", C.c_void_p), ("X_dev", C.c_void_p), ("C_dev", C.c_void_p), ("M", C.c_int), ("act", C.c_int), ("stage", C.c_int)]
+
+
+class Rotation(C.Structure):
+    """sptmm_rotation: Rotation(radians_per_position, interleaved) -- pair j of a head turns by position * radians_per_position[j]."""
+    _fields_ = [("pairs", C.c_int), ("interleaved", C.c_int), ("turns", C.c_uint64 * 128)]
+
+    def __init__(self, radians_per_position=(), interleaved=False):
+        super().__init__()
+        f = np.ascontiguousarray(radians_per_position, np.float64)
+        _ck(lib().sptmm_rotation_init(_p(f), f.size, int(bool(interleaved)), C.byref(self)))
+
+
+def _dev(x):
+    """A device address: a DeviceBuffer's, or an address as it is (None: NULL)."""
+    return x.ptr if isinstance(x, DeviceBuffer) else x
+
+
+def _stream(s):
+    """A Stream's handle, or a hipStream_t as it is (None: the default stream)."""
+    return s.handle if isinstance(s, Stream) else s
+
+
+class _Args(C.Structure):
+    """Argument block built from keywords; device buffers as DeviceBuffer or address."""
+
+    def __init__(self, **fields):
+        super().__init__()
+        for name, value in fields.items():
+            setattr(self, name, value)
+
+    def __setattr__(self, name, value):
+        if name not in self._names:
+            raise AttributeError("%s has no field %r" % (type(self).__name__, name))
+        if isinstance(value, Rotation):
+            object.__setattr__(self, "_held", value)  # the block points at it
+            value = C.pointer(value)
+        elif isinstance(value, DeviceBuffer):
+            value = value.ptr
+        super().__setattr__(name, value)
+
+
+class HeadsArgs(_Args):
+    """sptmm_heads_args (fields and rules: include/sptmm.h).  Keep the block and change its addresses from call to call."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("in_type", C.c_int), ("out_type", C.c_int), ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("v_out", C.c_void_p),
+                ("q_out_stride", C.c_int64), ("k_out_stride", C.c_int64), ("v_out_stride", C.c_int64),
+                ("tokens", C.c_int), ("q_heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("positions", C.c_void_p), ("kv_rows", C.c_void_p), ("kv_capacity", C.c_int64), ("q_gain", C.c_void_p), ("k_gain", C.c_void_p),
+                ("eps", C.c_float), ("rotation", C.POINTER(Rotation))]
+    _names = frozenset(n for n, _ in _fields_)
+
+
+class AttentionArgs(_Args):
+    """sptmm_attention_args (fields and rules: include/sptmm.h).  Keep the block and change its addresses from call to call."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("out_stride", C.c_int64), ("kv_rows", C.c_int64),
+                ("q_start", C.c_void_p), ("kv_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("batch", C.c_int), ("total_q", C.c_int), ("max_q", C.c_int), ("max_kv", C.c_int),
+                ("q_heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("type", C.c_int), ("scale", C.c_float)]
+    _names = frozenset(n for n, _ in _fields_)
 
 
 def lib_path() -> str:
@@ -137,6 +201,18 @@ def lib() -> C.CDLL:
         L.sptmm_weights_tune.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_double)]
         L.sptmm_stream_wait_event.argtypes = [C.c_void_p, C.c_void_p]
         L.sptmm_measure_sequence.argtypes = [C.POINTER(Step), C.c_int, C.c_int, C.c_int, C.c_void_p, C.POINTER(C.c_double)]
+        L.sptmm_adapters_create.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_void_p)]
+        L.sptmm_adapters_set.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_float, C.c_void_p]
+        L.sptmm_adapters_workspace_bytes.argtypes = [C.c_void_p, C.c_int]
+        L.sptmm_adapters_workspace_bytes.restype = C.c_size_t
+        L.sptmm_adapters_apply.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+        L.sptmm_adapters_free.argtypes = [C.c_void_p]
+        L.sptmm_adapters_free.restype = None
+        L.sptmm_rotation_init.argtypes = [C.c_void_p, C.c_int, C.c_int, C.POINTER(Rotation)]
+        L.sptmm_heads_norm_rotate.argtypes = [C.POINTER(HeadsArgs), C.c_void_p]
+        L.sptmm_attention_workspace_bytes.argtypes = [C.POINTER(AttentionArgs)]
+        L.sptmm_attention_workspace_bytes.restype = C.c_size_t
+        L.sptmm_attention.argtypes = [C.POINTER(AttentionArgs), C.c_void_p, C.c_size_t, C.c_void_p]
         _LIB = L
     return _LIB
 
@@ -501,6 +577,51 @@ def read_kernel(src: DeviceBuffer, nbytes: int, stream: Stream, launches: int = 
 
 def copy_kernel(dst: DeviceBuffer, src: DeviceBuffer, nbytes: int, stream: Stream | None = None):
     _ck(lib().sptmm_copy_kernel(dst.ptr, src.ptr, nbytes, stream.handle if stream else None))
+
+
+def heads_norm_rotate(args: HeadsArgs, stream: "Stream | int | None" = None):
+    """Norms of query and key heads, rotation by position, 16-bit heads out, keys and values to their cache rows (one launch)."""
+    _ck(lib().sptmm_heads_norm_rotate(C.byref(args), _stream(stream)))
+
+
+def attention_workspace_bytes(args: AttentionArgs) -> int:
+    return int(lib().sptmm_attention_workspace_bytes(C.byref(args)))
+
+
+def attention(args: AttentionArgs, workspace=None, workspace_bytes: int = 0, stream: "Stream | int | None" = None):
+    """Causal attention with grouped heads over packed sequences against a cache of rows."""
+    _ck(lib().sptmm_attention(C.byref(args), _dev(workspace), workspace_bytes, _stream(stream)))
+
+
+class Adapters:
+    """Low-rank adapters for one K x N projection, in slots (sptmm_adapters); buffers are DeviceBuffers or device addresses."""
+
+    def __init__(self, K: int, N: int, type: int, slots: int, max_rank: int):
+        self.handle = C.c_void_p()
+        self.K, self.N, self.type, self.slots, self.max_rank = K, N, type, slots, max_rank
+        _ck(lib().sptmm_adapters_create(K, N, type, slots, max_rank, C.byref(self.handle)))
+
+    def set(self, slot: int, A, B, rank: int, scale: float, stream: "Stream | int | None" = None):
+        """A [rank][K] and B [N][rank], 16-bit device buffers, into a slot (copied on `stream`); rank 0 empties it."""
+        _ck(lib().sptmm_adapters_set(self.handle, slot, _dev(A), _dev(B), rank, scale, _stream(stream)))
+
+    def workspace_bytes(self, M: int) -> int:
+        return int(lib().sptmm_adapters_workspace_bytes(self.handle, M))
+
+    def apply(self, X, row_slot, M: int, base, Y, workspace, workspace_bytes: int, stream: "Stream | int | None" = None):
+        """Y[m] = base[m] + scale * B (A X[m]) with the adapter in slot row_slot[m] (int32 on the device; outside: none); base may be Y or None."""
+        _ck(lib().sptmm_adapters_apply(self.handle, _dev(X), _dev(row_slot), M, _dev(base), _dev(Y), _dev(workspace), workspace_bytes, _stream(stream)))
+
+    def free(self):
+        if self.handle:
+            lib().sptmm_adapters_free(self.handle)
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
 
 
 class Weights:

@@ -1,0 +1,355 @@
+// Low-rank adapters of many requests beside one shared projection:
+//
+//   Y[m][n] = base[m][n] + scale_s * sum_r B_s[n][r] * h[m][r],   h[m][r] = sum_k A_s[r][k] X[m][k],   s = row_slot[m]
+//
+// Two launches.  The first makes h: 16 rows of X against 16 ranks of A per matrix instruction (16-bit operands, 32-bit
+// sums), the rows' contraction over K split over wavefronts and workgroups.  The second adds up the splits' partial sums in
+// their order and multiplies by B on the 32-bit matrix instruction: h is never rounded to 16 bits -- outputs are 32-bit
+// floats, and a rounded h would cost them fifteen of their bits -- and B's 16-bit values are exact in 32.
+//
+// Rows come in any order of slots.  A tile of 16 rows is walked once per distinct slot in it (found by ballots, no sorting
+// pass); a matrix column is a row of X and stays in its lanes throughout, so rows of other slots are left out by a select
+// and never by a product with zero: an infinity in one adapter's weights reaches its own rows only.
+//
+// Both weights sit in the order in which a wavefront reads them, 1 KiB per load instruction (adapters_pack_kernel).
+#include <cmath>
+
+#include "internal.hpp"
+#include "lanes.hpp"
+
+struct sptmm_adapters {
+    int K, N, type, slots, max_rank;
+    int k_steps;     // steps of 32 along K (the last one padded with zeros)
+    int n_pairs;     // pairs of 16 columns
+    int max_chunks;  // chunks of 16 ranks a slot has room for
+    int device, compute_units;
+    uint16_t *A, *B;  // [slot]: [chunk][k_step][64 lanes][8] and [n_pair][chunk][64 lanes][8], packed by the chunks in use
+    int *chunks;      // [slot] chunks of 16 ranks in use; 0: empty
+    float *scale;     // [slot]
+};
+
+namespace sptmm {
+namespace {
+
+typedef unsigned short u16;
+typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+
+template <int T> __device__ __forceinline__ f32x4 mfma16(u16x8 a, u16x8 b, f32x4 c)
+{
+    if constexpr (T == SPTMM_X_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <int T> __device__ __forceinline__ float widen(u16 b)
+{
+    if constexpr (T == SPTMM_X_F16) return (float)__builtin_bit_cast(_Float16, b);
+    return __builtin_bit_cast(float, (unsigned)b << 16);
+}
+
+struct AdapterArgs {
+    const u16 *X, *A, *B;
+    const int *row_slot, *chunks;
+    const float *scale, *base;
+    float *h, *Y;
+    int M, K, N, slots, k_steps, n_pairs, max_chunks, tiles, splits;
+};
+
+// ------------------------------------------------------------------------------------------------ weights into place
+// One thread per stored value.  A lane of the first product's operand holds rank lane % 16, k = 8 * (lane / 16) + e of a step
+// of 32; of the second's, column lane % 16 (e < 4) or 16 + lane % 16 (e >= 4) of a pair, rank 4 * (lane / 16) + e % 4 of a chunk.
+__global__ void __launch_bounds__(256) adapters_pack_kernel(const u16 *A, const u16 *B, u16 *pA, u16 *pB, int *chunk_of, float *scale_of, int slot, int rank, float scale, int K,
+                                                            int N, int k_steps, int n_pairs, int chunks)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i == 0) chunk_of[slot] = chunks, scale_of[slot] = scale;
+    const int64_t na = (int64_t)chunks * k_steps * 512, nb = (int64_t)n_pairs * chunks * 512;
+    const int e = (int)(i & 7), lane = (int)(i >> 3) & 63;
+    if (i < na) {
+        const int step = (int)((i >> 9) % k_steps), c = (int)((i >> 9) / k_steps);
+        const int r = 16 * c + (lane & 15), k = 32 * step + 8 * (lane >> 4) + e;
+        pA[i] = r < rank && k < K ? A[(int64_t)r * K + k] : (u16)0;
+    }
+    if (i < nb) {
+        const int c = (int)((i >> 9) % chunks), pair = (int)((i >> 9) / chunks);
+        const int n = 32 * pair + 16 * (e >> 2) + (lane & 15), r = 16 * c + 4 * (lane >> 4) + (e & 3);
+        pB[i] = r < rank && n < N ? B[(int64_t)n * rank + r] : (u16)0;
+    }
+}
+
+// the distinct slots of the rows that the low 16 lanes hold: call with the mask of rows not yet served
+__device__ __forceinline__ int next_slot(int slot, unsigned long long &left)
+{
+    const int s = __builtin_amdgcn_readlane(slot, __builtin_ctzll(left));
+    left &= ~__ballot(slot == s);
+    return s;
+}
+
+// ------------------------------------------------------------------------------------------------ h = X A^T
+constexpr int SHRINK_WAVES = 8;
+constexpr int CHUNKS_AT_ONCE = 4;  // chunks of 16 ranks summed in one walk over K (X is read once per walk)
+
+// Workgroup (tile of 16 rows, split of K, ordinal of a distinct slot in the tile): eight wavefronts take every eighth step of the
+// split's range of K, and add their sums through the LDS in wavefront order.  ONE: a workgroup serves one slot of its tile (few
+// rows: slots spread over workgroups); else it walks them all.
+template <int T, bool ONE> __global__ void __launch_bounds__(SHRINK_WAVES * 64) adapters_shrink_kernel(const AdapterArgs p)
+{
+    __shared__ __attribute__((aligned(16))) f32x4 sums[SHRINK_WAVES][CHUNKS_AT_ONCE][64];
+    const int tile = blockIdx.x, split = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m = tile * 16 + (lane & 15);
+    int slot = m < p.M ? p.row_slot[m] : -1;
+    if (slot < 0 || slot >= p.slots) slot = -1;
+    unsigned long long left = __ballot(slot >= 0) & 0xffff;
+    if (ONE)
+        for (int o = blockIdx.z; o > 0 && left; --o) next_slot(slot, left);
+    // this workgroup's steps of K
+    const int per = (p.k_steps + p.splits - 1) / p.splits, step0 = split * per, step1 = min(p.k_steps, step0 + per);
+    const u16 *x_row = p.X + (int64_t)min(m, p.M - 1) * p.K + 8 * (lane >> 4);
+    while (left) {
+        const int s = next_slot(slot, left), chunks = p.chunks[s];
+        for (int c0 = 0; c0 < chunks; c0 += CHUNKS_AT_ONCE) {
+            const int nc = min(CHUNKS_AT_ONCE, chunks - c0);
+            f32x4 acc[CHUNKS_AT_ONCE];
+#pragma unroll
+            for (int c = 0; c < CHUNKS_AT_ONCE; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const u16 *a = p.A + (((int64_t)s * p.max_chunks + c0) * p.k_steps) * 512 + lane * 8;
+#pragma unroll 4
+            for (int step = step0 + wave; step < step1; step += SHRINK_WAVES) {
+                u16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (32 * step + 8 * (lane >> 4) < p.K) x = *reinterpret_cast<const u16x8 *>(x_row + 32 * step);
+#pragma unroll
+                for (int c = 0; c < CHUNKS_AT_ONCE; ++c)
+                    if (c < nc) acc[c] = mfma16<T>(*reinterpret_cast<const u16x8 *>(a + ((int64_t)c * p.k_steps + step) * 512), x, acc[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < CHUNKS_AT_ONCE; ++c)
+                if (c < nc) sums[wave][c][lane] = acc[c];
+            __syncthreads();
+            if (wave < nc) {
+                f32x4 t = sums[0][wave][lane];
+                for (int w = 1; w < SHRINK_WAVES; ++w) t += sums[w][wave][lane];
+                if (slot == s) reinterpret_cast<f32x4 *>(p.h)[(((int64_t)split * p.tiles + tile) * p.max_chunks + c0 + wave) * 64 + lane] = t;
+            }
+            __syncthreads();
+        }
+        if (ONE) break;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ Y = base + scale * h B^T
+// A wavefront takes 16 * RT rows and 32 columns.  ONE: only the rows of one distinct slot of its tile (and, the first of them,
+// the rows without a slot); else all slots of its rows.
+template <int T, int RT, bool ONE> __global__ void __launch_bounds__(256) adapters_expand_kernel(const AdapterArgs p)
+{
+    const int lane = threadIdx.x & 63, pair = blockIdx.y * 4 + (threadIdx.x >> 6), tile0 = blockIdx.x * RT;
+    if (pair >= p.n_pairs) return;
+    int slot[RT];
+    bool write[RT];
+    unsigned long long left[RT], any = 0;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int m = (tile0 + t) * 16 + (lane & 15);
+        int s = m < p.M ? p.row_slot[m] : -1;
+        if (s < 0 || s >= p.slots) s = -1;
+        slot[t] = s;
+        left[t] = __ballot(s >= 0) & 0xffff;
+        write[t] = m < p.M;
+        any |= left[t];
+    }
+    if (ONE) {
+        for (int o = blockIdx.z; o > 0 && left[0]; --o) next_slot(slot[0], left[0]);
+        if (!left[0] && blockIdx.z) return;
+        const int mine = left[0] ? __builtin_amdgcn_readlane(slot[0], __builtin_ctzll(left[0])) : -2;
+        write[0] = write[0] && (slot[0] == mine || (blockIdx.z == 0 && slot[0] < 0));
+        left[0] &= __ballot(slot[0] == mine);
+    }
+    const int n0 = pair * 32 + 4 * (lane >> 4);
+    const bool second = pair * 32 + 16 < p.N;  // (an odd number of 16-column groups: the last pair has one)
+    f32x4 acc[RT][2];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int64_t at = (int64_t)((tile0 + t) * 16 + (lane & 15)) * p.N + n0;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            acc[t][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (p.base && write[t] && (g == 0 || second)) acc[t][g] = *reinterpret_cast<const f32x4 *>(p.base + at + 16 * g);
+        }
+    }
+#pragma unroll
+    for (int t0 = 0; t0 < RT; ++t0) {
+        while (left[t0]) {  // distinct slots of all the rows: those of a later tile are served with the first tile that has them
+            const int s = next_slot(slot[t0], left[t0]), chunks = p.chunks[s];
+            bool has[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const unsigned long long b = __ballot(slot[t] == s) & 0xffff;
+                has[t] = t >= t0 && b;
+                if (t > t0) left[t] &= ~b;
+            }
+            const float scale = p.scale[s];
+            for (int c = 0; c < chunks; ++c) {
+                const u16x8 b = *reinterpret_cast<const u16x8 *>(p.B + ((int64_t)s * p.n_pairs * p.max_chunks + (int64_t)pair * chunks + c) * 512 + lane * 8);
+                float bw[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) bw[e] = widen<T>(b[e]);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    if (!has[t]) continue;
+                    const f32x4 *hp = reinterpret_cast<const f32x4 *>(p.h) + ((int64_t)(tile0 + t) * p.max_chunks + c) * 64 + lane;
+                    f32x4 h = {0.f, 0.f, 0.f, 0.f};
+                    if (slot[t] == s) {
+                        h = hp[0];
+                        for (int k = 1; k < p.splits; ++k) h += hp[(int64_t)k * p.tiles * p.max_chunks * 64];
+                        h *= scale;
+                    }
+                    f32x4 y0 = acc[t][0], y1 = acc[t][1];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        y0 = __builtin_amdgcn_mfma_f32_16x16x4f32(bw[e], h[e], y0, 0, 0, 0);
+                        y1 = __builtin_amdgcn_mfma_f32_16x16x4f32(bw[4 + e], h[e], y1, 0, 0, 0);
+                    }
+                    if (slot[t] == s) acc[t][0] = y0, acc[t][1] = y1;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int64_t at = (int64_t)((tile0 + t) * 16 + (lane & 15)) * p.N + n0;
+        if (write[t]) {
+            *reinterpret_cast<f32x4 *>(p.Y + at) = acc[t][0];
+            if (second) *reinterpret_cast<f32x4 *>(p.Y + at + 16) = acc[t][1];
+        }
+    }
+}
+
+int hip_fail(hipError_t e, const char *what) { return fail(SPTMM_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e); }
+
+// Up to this many rows the distinct slots of a tile go to workgroups of their own (decode: every row may have another one, and a
+// workgroup that walks sixteen waits for sixteen chains of loads); beyond it, prompts, a tile rarely has more than two.
+constexpr int SPREAD_ROWS = 128;
+
+int ordinals(int M) { return M <= SPREAD_ROWS ? (M < 16 ? M : 16) : 1; }
+
+// splits of K over workgroups: enough of them to fill the chip, each wavefront with two steps of 32 at least
+int splits_of(const sptmm_adapters *a, int M)
+{
+    const int tiles = (M + 15) / 16, groups = tiles * ordinals(M);
+    const int want = (a->compute_units + groups - 1) / groups, most = (a->k_steps + 2 * SHRINK_WAVES - 1) / (2 * SHRINK_WAVES);
+    return want < 1 ? 1 : want < most ? want : most;
+}
+
+size_t need(const sptmm_adapters *a, int M)
+{
+    return (size_t)splits_of(a, M) * ((M + 15) / 16) * a->max_chunks * 64 * 16;
+}
+
+int check_device(const sptmm_adapters *a)
+{
+    int dev = -1;
+    const hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return hip_fail(e, "hipGetDevice");
+    if (dev != a->device) return fail(SPTMM_ERR_INVALID, "the adapters live on device %d but device %d is current", a->device, dev);
+    return SPTMM_OK;
+}
+
+template <int T> void launch_apply(const AdapterArgs &p, int ord, hipStream_t st)
+{
+    if (ord > 1 || p.M <= SPREAD_ROWS) {
+        hipLaunchKernelGGL((adapters_shrink_kernel<T, true>), dim3(p.tiles, p.splits, ord), dim3(SHRINK_WAVES * 64), 0, st, p);
+        hipLaunchKernelGGL((adapters_expand_kernel<T, 1, true>), dim3(p.tiles, (p.n_pairs + 3) / 4, ord), dim3(256), 0, st, p);
+    } else {
+        hipLaunchKernelGGL((adapters_shrink_kernel<T, false>), dim3(p.tiles, p.splits, 1), dim3(SHRINK_WAVES * 64), 0, st, p);
+        hipLaunchKernelGGL((adapters_expand_kernel<T, 4, false>), dim3((p.tiles + 3) / 4, (p.n_pairs + 3) / 4, 1), dim3(256), 0, st, p);
+    }
+}
+
+}  // namespace
+}  // namespace sptmm
+
+using namespace sptmm;
+
+extern "C" void sptmm_adapters_free(sptmm_adapters *a)
+{
+    if (!a) return;
+    if (a->A) (void)hipFree(a->A);
+    if (a->B) (void)hipFree(a->B);
+    if (a->chunks) (void)hipFree(a->chunks);
+    if (a->scale) (void)hipFree(a->scale);
+    delete a;
+}
+
+extern "C" int sptmm_adapters_create(int K, int N, int type, int slots, int max_rank, sptmm_adapters **out)
+{
+    if (!out) return fail(SPTMM_ERR_INVALID, "null pointer");
+    if (K < 16 || N < 16 || K % 16 || N % 16) return fail(SPTMM_ERR_INVALID, "K and N must be positive multiples of 16");
+    if (K > (1 << 20) || N > (1 << 20)) return fail(SPTMM_ERR_INVALID, "K and N must be at most 2^20");
+    if (type != SPTMM_X_F16 && type != SPTMM_X_BF16) return fail(SPTMM_ERR_INVALID, "type must be SPTMM_X_F16 or SPTMM_X_BF16");
+    if (slots < 1 || slots > 65536) return fail(SPTMM_ERR_INVALID, "slots must be 1..65536");
+    if (max_rank < 1 || max_rank > 256) return fail(SPTMM_ERR_INVALID, "max_rank must be 1..256");
+    sptmm_adapters *a = new (std::nothrow) sptmm_adapters();
+    if (!a) return fail(SPTMM_ERR_NOMEM, "out of host memory");
+    a->K = K, a->N = N, a->type = type, a->slots = slots, a->max_rank = max_rank;
+    a->k_steps = (K + 31) / 32, a->n_pairs = (N + 31) / 32, a->max_chunks = (max_rank + 15) / 16;
+    const size_t per_a = (size_t)a->max_chunks * a->k_steps * 1024, per_b = (size_t)a->max_chunks * a->n_pairs * 1024;
+    hipError_t e = hipGetDevice(&a->device);
+    if (e == hipSuccess) e = hipDeviceGetAttribute(&a->compute_units, hipDeviceAttributeMultiprocessorCount, a->device);
+    if (e == hipSuccess) e = hipMalloc((void **)&a->A, per_a * slots);
+    if (e == hipSuccess) e = hipMalloc((void **)&a->B, per_b * slots);
+    if (e == hipSuccess) e = hipMalloc((void **)&a->chunks, sizeof(int) * slots);
+    if (e == hipSuccess) e = hipMalloc((void **)&a->scale, sizeof(float) * slots);
+    if (e == hipSuccess) e = hipMemset(a->chunks, 0, sizeof(int) * slots);
+    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (e != hipSuccess) {
+        sptmm_adapters_free(a);
+        return e == hipErrorOutOfMemory ? fail(SPTMM_ERR_NOMEM, "out of device memory for %d adapters", slots) : hip_fail(e, "sptmm_adapters_create");
+    }
+    *out = a;
+    return SPTMM_OK;
+}
+
+extern "C" int sptmm_adapters_set(sptmm_adapters *a, int slot, const uint16_t *A, const uint16_t *B, int rank, float scale, void *stream)
+{
+    if (!a) return fail(SPTMM_ERR_INVALID, "null pointer");
+    if (slot < 0 || slot >= a->slots) return fail(SPTMM_ERR_INVALID, "slot %d out of range (have %d)", slot, a->slots);
+    if (rank < 0 || rank > a->max_rank) return fail(SPTMM_ERR_INVALID, "rank must be 0 (empty the slot) to %d", a->max_rank);
+    if (rank && (!A || !B)) return fail(SPTMM_ERR_INVALID, "null pointer");
+    if (!std::isfinite(scale)) return fail(SPTMM_ERR_INVALID, "scale must be finite");
+    if (int rc = check_device(a)) return rc;
+    const int chunks = (rank + 15) / 16;
+    const int64_t n = (int64_t)chunks * 512 * std::max(a->k_steps, a->n_pairs);
+    u16 *pA = a->A + (size_t)slot * a->max_chunks * a->k_steps * 512, *pB = a->B + (size_t)slot * a->max_chunks * a->n_pairs * 512;
+    hipLaunchKernelGGL(adapters_pack_kernel, dim3((unsigned)std::max<int64_t>(1, (n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, A, B, pA, pB, a->chunks, a->scale, slot, rank,
+                       scale, a->K, a->N, a->k_steps, a->n_pairs, chunks);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? SPTMM_OK : hip_fail(e, "adapters_pack_kernel launch");
+}
+
+extern "C" size_t sptmm_adapters_workspace_bytes(const sptmm_adapters *a, int M)
+{
+    if (!a || M < 1) return 0;
+    return need(a, M);
+}
+
+extern "C" int sptmm_adapters_apply(const sptmm_adapters *a, const uint16_t *X, const int32_t *row_slot, int M, const float *base, float *Y, void *workspace,
+                                    size_t workspace_bytes, void *stream)
+{
+    if (!a || !X || !row_slot || !Y || !workspace) return fail(SPTMM_ERR_INVALID, "null pointer");
+    if (M < 1) return fail(SPTMM_ERR_INVALID, "M must be at least 1");
+    if (M > (1 << 24)) return fail(SPTMM_ERR_INVALID, "M must be at most 2^24");
+    if (((uintptr_t)X | (uintptr_t)base | (uintptr_t)Y | (uintptr_t)workspace) & 15) return fail(SPTMM_ERR_INVALID, "X, base, Y and the workspace must be aligned to 16 bytes");
+    if ((uintptr_t)row_slot & 3) return fail(SPTMM_ERR_INVALID, "row_slot must be aligned to 4 bytes");
+    if (workspace_bytes < need(a, M)) return fail(SPTMM_ERR_INVALID, "the workspace has %zu bytes, %zu are needed", workspace_bytes, need(a, M));
+    if (int rc = check_device(a)) return rc;
+    AdapterArgs p{};
+    p.X = X, p.A = a->A, p.B = a->B, p.row_slot = row_slot, p.chunks = a->chunks, p.scale = a->scale, p.base = base, p.h = (float *)workspace, p.Y = Y;
+    p.M = M, p.K = a->K, p.N = a->N, p.slots = a->slots, p.k_steps = a->k_steps, p.n_pairs = a->n_pairs, p.max_chunks = a->max_chunks;
+    p.tiles = (M + 15) / 16, p.splits = splits_of(a, M);
+    const int ord = ordinals(M);
+    a->type == SPTMM_X_F16 ? launch_apply<SPTMM_X_F16>(p, ord, (hipStream_t)stream) : launch_apply<SPTMM_X_BF16>(p, ord, (hipStream_t)stream);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? SPTMM_OK : hip_fail(e, "adapters kernels launch");
+}

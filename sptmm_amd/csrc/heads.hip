@@ -1,0 +1,296 @@
+// What lies between a decoder layer's q+k+v projection and its attention, in one pass: norms of the query and key heads,
+// the rotation by position, the rounding to 16 bits, and the scatter of key and value heads to their cache rows.
+//
+//   x' = x * rsqrt(mean(x^2) + eps) * gain              (query and key heads; without a gain: x' = x)
+//   (a, b) -> (a cos w - b sin w, b cos w + a sin w)      pair j of the first 2 * pairs elements, w = position * frequency_j
+//
+// The angle is kept as a fraction of a turn in 64-bit fixed point: turns_j = frequency_j / 2 pi as a fraction of 2^64, and
+// position * turns_j mod 2^64 is the phase, exact to position * 2^-65 turns however far the position -- no table of sines
+// to read, and no loss at far positions, where a product in 32 bits is off by position * 2^-24 radians.
+// Everything is computed in 32 bits and rounded once, to nearest even, on the way out.
+//
+// The pass is bound by its bytes.  A lane holds four pairs (eight elements: two loads of 16 bytes from float rows), so a
+// head of 128 takes 16 lanes and a wavefront handles four heads at a time; the sines of a token's four pairs stay in the
+// lane's registers while it walks the token's heads.
+#include <cmath>
+
+#include "internal.hpp"
+#include "lanes.hpp"
+
+namespace sptmm {
+namespace {
+
+typedef unsigned short u16;
+typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+
+struct HeadsParams {
+    const void *q, *k, *v;
+    void *q_out, *k_out, *v_out;
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride, v_out_stride, kv_capacity;
+    const int *positions, *kv_rows;
+    const float *q_gain, *k_gain;
+    float eps, inv_dim;
+    int tokens, q_heads, kv_heads, heads, dim, pairs;  // heads: query + key + value heads of a token (value heads only where v is given)
+    int log_lanes;                                     // 1 << log_lanes lanes per head
+    int parts, per_part;                               // a token's heads are shared by `parts` wavefronts, `per_part` heads each
+    uint64_t turns[SPTMM_MAX_ROTATED_PAIRS];
+};
+
+template <int T> __device__ __forceinline__ float widen(u16 b)
+{
+    if constexpr (T == SPTMM_X_F16) return (float)__builtin_bit_cast(_Float16, b);
+    return __builtin_bit_cast(float, (unsigned)b << 16);
+}
+template <int T> __device__ __forceinline__ u16 narrow(float x)
+{
+    if constexpr (T == SPTMM_X_F16) return __builtin_bit_cast(u16, (_Float16)x);
+    return __builtin_bit_cast(u16, (__bf16)x);
+}
+
+// element index of the first (w = 0) and second (w = 1) element of pair slot s
+template <bool INTER> __device__ __forceinline__ int element(const HeadsParams &p, int s, int w)
+{
+    if (INTER) return 2 * s + w;
+    const int rest = p.dim / 2 - p.pairs;  // the elements behind the rotated ones are held as pairs too, at angle 0
+    return s < p.pairs ? s + w * p.pairs : 2 * p.pairs + (s - p.pairs) + w * rest;
+}
+
+template <int IN, bool INTER, bool WIDE> __device__ __forceinline__ void load8(const HeadsParams &p, const void *row, int s0, int slots, float (&x)[2][4])
+{
+    if constexpr (WIDE) {
+        // four consecutive pair slots: two runs of four elements (apart: two loads; neighbouring pairs: one run of eight)
+        const int e0 = INTER ? 2 * s0 : element<INTER>(p, s0, 0), e1 = INTER ? 2 * s0 + 4 : element<INTER>(p, s0, 1);
+        float r[2][4];
+        if constexpr (IN == SPTMM_X_F32) {
+            const f32x4 a = *reinterpret_cast<const f32x4 *>((const float *)row + e0), b = *reinterpret_cast<const f32x4 *>((const float *)row + e1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[0][i] = a[i], r[1][i] = b[i];
+        } else {
+            const u16x4 a = *reinterpret_cast<const u16x4 *>((const u16 *)row + e0), b = *reinterpret_cast<const u16x4 *>((const u16 *)row + e1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[0][i] = widen<IN>(a[i]), r[1][i] = widen<IN>(b[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[0][i] = INTER ? r[i / 2][2 * (i & 1)] : r[0][i];
+            x[1][i] = INTER ? r[i / 2][2 * (i & 1) + 1] : r[1][i];
+        }
+    } else {
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[w][i] = 0.f;
+                if (s0 + i < slots) {
+                    const int e = element<INTER>(p, s0 + i, w);
+                    if constexpr (IN == SPTMM_X_F32)
+                        x[w][i] = ((const float *)row)[e];
+                    else
+                        x[w][i] = widen<IN>(((const u16 *)row)[e]);
+                }
+            }
+    }
+}
+
+template <int OUT, bool INTER, bool WIDE> __device__ __forceinline__ void store8(const HeadsParams &p, u16 *row, int s0, int slots, const float (&x)[2][4])
+{
+    if constexpr (WIDE) {
+        const int e0 = INTER ? 2 * s0 : element<INTER>(p, s0, 0), e1 = INTER ? 2 * s0 + 4 : element<INTER>(p, s0, 1);
+        u16x4 a, b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[i] = narrow<OUT>(INTER ? x[i & 1][i / 2] : x[0][i]);
+            b[i] = narrow<OUT>(INTER ? x[i & 1][2 + i / 2] : x[1][i]);
+        }
+        *reinterpret_cast<u16x4 *>(row + e0) = a;
+        *reinterpret_cast<u16x4 *>(row + e1) = b;
+    } else {
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (s0 + i < slots) row[element<INTER>(p, s0 + i, w)] = narrow<OUT>(x[w][i]);
+    }
+}
+
+// IN: type of the rows; OUT: type of the heads written; INTER: pairs of neighbours (2j, 2j+1), else of halves (j, j + pairs);
+// WIDE: every run of four elements lies aligned for one load or store
+template <int IN, int OUT, bool INTER, bool WIDE> __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p)
+{
+    const int lane = threadIdx.x & 63;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= (int64_t)p.tokens * p.parts) return;
+    const int t = (int)(unit / p.parts), part = (int)(unit - (int64_t)t * p.parts);
+    const int per_wave = 64 >> p.log_lanes, sub = lane >> p.log_lanes, s0 = (lane & ((1 << p.log_lanes) - 1)) * 4, slots = p.dim / 2;
+    const bool mine = s0 < slots;
+    const int first = part * p.per_part, end = min(p.heads, first + p.per_part);
+
+    float cs[4], sn[4];
+    {
+        const int pos = p.positions ? p.positions[t] : t;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            cs[i] = 1.f, sn[i] = 0.f;
+            if (s0 + i < p.pairs) {
+                // the phase as a signed fraction of a turn: 32 of its 64 bits are more than a float holds
+                const uint64_t phase = (uint64_t)(int64_t)pos * p.turns[s0 + i];
+                const float half_turns = (float)(int)(phase >> 32) * 0x1p-31f;
+                sincospif(half_turns, &sn[i], &cs[i]);
+            }
+        }
+    }
+    int64_t kv_row = p.kv_rows ? p.kv_rows[t] : t;
+    const bool kept = kv_row >= 0 && kv_row < p.kv_capacity;
+
+    constexpr int ESZ = IN == SPTMM_X_F32 ? 4 : 2;
+    for (int h0 = first; h0 < end; h0 += per_wave) {
+        const int h = h0 + sub;
+        const bool is_q = h < p.q_heads, is_v = h >= p.q_heads + p.kv_heads, live = mine && h < end;
+        const int at = is_q ? h : is_v ? h - p.q_heads - p.kv_heads : h - p.q_heads;
+        const char *src = (const char *)(is_q ? p.q : is_v ? p.v : p.k) + ((int64_t)t * (is_q ? p.q_stride : is_v ? p.v_stride : p.k_stride) + (int64_t)at * p.dim) * ESZ;
+        float x[2][4] = {{0.f}};
+        if (live) load8<IN, INTER, WIDE>(p, src, s0, slots, x);
+        const float *gain = is_q ? p.q_gain : p.k_gain;
+        if (gain && !is_v) {  // (lanes of one head agree)
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum = fmaf(x[w][i], x[w][i], sum);
+            for (int o = 1; o < 1 << p.log_lanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
+            const float r = 1.0f / sqrtf(fmaf(sum, p.inv_dim, p.eps));
+            if (live) {
+                float g[2][4];
+                load8<SPTMM_X_F32, INTER, WIDE>(p, gain, s0, slots, g);
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[w][i] = x[w][i] * r * g[w][i];
+            }
+        }
+        if (!is_v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (s0 + i < p.pairs) {
+                    const float a = x[0][i], b = x[1][i];
+                    x[0][i] = a * cs[i] - b * sn[i];
+                    x[1][i] = b * cs[i] + a * sn[i];
+                }
+            }
+        if (live && (is_q || kept)) {
+            u16 *dst = (u16 *)(is_q ? p.q_out : is_v ? p.v_out : p.k_out) +
+                       ((is_q ? (int64_t)t * p.q_out_stride : kv_row * (is_v ? p.v_out_stride : p.k_out_stride)) + (int64_t)at * p.dim);
+            store8<OUT, INTER, WIDE>(p, dst, s0, slots, x);
+        }
+    }
+}
+
+template <int IN, int OUT> void launch_in_out(const HeadsParams &p, bool inter, bool wide, int blocks, hipStream_t st)
+{
+    const auto kernel = inter ? (wide ? heads_kernel<IN, OUT, true, true> : heads_kernel<IN, OUT, true, false>)
+                              : (wide ? heads_kernel<IN, OUT, false, true> : heads_kernel<IN, OUT, false, false>);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, st, p);
+}
+
+bool aligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+}  // namespace
+}  // namespace sptmm
+
+using namespace sptmm;
+
+extern "C" int sptmm_rotation_init(const double *radians_per_position, int pairs, int interleaved, sptmm_rotation *out)
+{
+    if (!out || (pairs > 0 && !radians_per_position)) return fail(SPTMM_ERR_INVALID, "null pointer");
+    if (pairs < 0 || pairs > SPTMM_MAX_ROTATED_PAIRS) return fail(SPTMM_ERR_INVALID, "pairs must be 0..%d", SPTMM_MAX_ROTATED_PAIRS);
+    sptmm_rotation r{};
+    r.pairs = pairs;
+    r.interleaved = interleaved ? 1 : 0;
+    for (int j = 0; j < pairs; ++j) {
+        const long double turn = (long double)radians_per_position[j] / 6.283185307179586476925286766559005768L;
+        if (!std::isfinite((double)turn)) return fail(SPTMM_ERR_INVALID, "the frequency of pair %d is not finite", j);
+        const long double whole = floorl(turn), f = (turn - whole) * 18446744073709551616.0L;  // fraction of a turn, of 2^64
+        r.turns[j] = f >= 18446744073709551615.0L ? UINT64_MAX : (uint64_t)(f + 0.5L);
+    }
+    *out = r;
+    return SPTMM_OK;
+}
+
+extern "C" int sptmm_heads_norm_rotate(const sptmm_heads_args *a, void *stream)
+{
+    if (!a) return fail(SPTMM_ERR_INVALID, "null pointer");
+    if (a->tokens < 0 || a->q_heads < 0 || a->kv_heads < 0 || a->q_heads + a->kv_heads < 1 || a->q_heads > 65535 || a->kv_heads > 65535)
+        return fail(SPTMM_ERR_INVALID, "tokens, q_heads and kv_heads must not be negative, at most 65535 heads, and not both counts zero");
+    if (a->head_dim < 2 || a->head_dim > 256 || a->head_dim % 2) return fail(SPTMM_ERR_INVALID, "head_dim must be even, 2..256");
+    if (a->in_type != SPTMM_X_F16 && a->in_type != SPTMM_X_BF16 && a->in_type != SPTMM_X_F32)
+        return fail(SPTMM_ERR_INVALID, "in_type must be SPTMM_X_F16, SPTMM_X_BF16 or SPTMM_X_F32");
+    if (a->out_type != SPTMM_X_F16 && a->out_type != SPTMM_X_BF16) return fail(SPTMM_ERR_INVALID, "out_type must be SPTMM_X_F16 or SPTMM_X_BF16");
+    if (a->tokens == 0) return SPTMM_OK;
+    const bool has_v = a->v != nullptr;
+    if ((a->q_heads && (!a->q || !a->q_out)) || (a->kv_heads && (!a->k || !a->k_out)) || (a->kv_heads && has_v && !a->v_out))
+        return fail(SPTMM_ERR_INVALID, "null pointer");
+    const int64_t q_row = (int64_t)a->q_heads * a->head_dim, kv_row = (int64_t)a->kv_heads * a->head_dim;
+    if (a->q_stride < q_row || a->q_out_stride < q_row || a->k_stride < kv_row || a->k_out_stride < kv_row ||
+        (has_v && (a->v_stride < kv_row || a->v_out_stride < kv_row)))
+        return fail(SPTMM_ERR_INVALID, "a row stride is shorter than its row of heads");
+    if (a->kv_capacity < 0) return fail(SPTMM_ERR_INVALID, "kv_capacity must not be negative");
+    const sptmm_rotation *rot = a->rotation;
+    if (rot && (rot->pairs < 0 || rot->pairs > SPTMM_MAX_ROTATED_PAIRS || 2 * rot->pairs > a->head_dim))
+        return fail(SPTMM_ERR_INVALID, "the rotation has %d pairs, more than half of head_dim %d", rot->pairs, a->head_dim);
+    if ((a->q_gain || a->k_gain) && !(a->eps >= 0.f && a->eps < 1e30f)) return fail(SPTMM_ERR_INVALID, "eps must be finite and not negative");
+    // elements and their natural alignment
+    const size_t isz = a->in_type == SPTMM_X_F32 ? 4 : 2;
+    const void *ins[3] = {a->q, a->k, a->v}, *outs[3] = {a->q_out, a->k_out, a->v_out}, *words[4] = {a->positions, a->kv_rows, a->q_gain, a->k_gain};
+    for (const void *x : ins)
+        if (!aligned(x, isz)) return fail(SPTMM_ERR_INVALID, "rows must be aligned to their elements");
+    for (const void *x : outs)
+        if (!aligned(x, 2)) return fail(SPTMM_ERR_INVALID, "rows must be aligned to their elements");
+    for (const void *x : words)
+        if (!aligned(x, 4)) return fail(SPTMM_ERR_INVALID, "positions, kv_rows and gains must be aligned to 4 bytes");
+
+    HeadsParams p{};
+    p.q = a->q, p.k = a->k, p.v = a->v, p.q_out = a->q_out, p.k_out = a->k_out, p.v_out = a->v_out;
+    p.q_stride = a->q_stride, p.k_stride = a->k_stride, p.v_stride = a->v_stride;
+    p.q_out_stride = a->q_out_stride, p.k_out_stride = a->k_out_stride, p.v_out_stride = a->v_out_stride;
+    p.kv_capacity = a->kv_capacity;
+    p.positions = a->positions, p.kv_rows = a->kv_rows, p.q_gain = a->q_gain, p.k_gain = a->k_gain;
+    p.eps = a->eps, p.inv_dim = 1.0f / (float)a->head_dim;
+    p.tokens = a->tokens, p.q_heads = a->q_heads, p.kv_heads = a->kv_heads, p.dim = a->head_dim;
+    p.heads = a->q_heads + a->kv_heads * (has_v ? 2 : 1);
+    const bool inter = rot && rot->interleaved;
+    if (rot) {
+        p.pairs = rot->pairs;
+        for (int j = 0; j < rot->pairs; ++j) p.turns[j] = rot->turns[j];
+    }
+    p.log_lanes = 0;
+    while ((8 << p.log_lanes) < a->head_dim) ++p.log_lanes;
+    const int per_wave = 64 >> p.log_lanes, rounds = (p.heads + per_wave - 1) / per_wave;
+    // One wavefront per round of heads while that leaves the chip's wavefront slots unfilled (a lone token: one round of
+    // latency instead of eight), one wavefront per token once there are enough tokens (the sines are computed once).
+    p.parts = a->tokens >= 2048 ? 1 : rounds;
+    const int rounds_per_part = (rounds + p.parts - 1) / p.parts;
+    p.per_part = rounds_per_part * per_wave;
+    const int64_t units = (int64_t)a->tokens * p.parts;
+    if (units > (int64_t)4 * 0x7fffffff) return fail(SPTMM_ERR_INVALID, "too many tokens");
+    const int blocks = (int)((units + 3) / 4);
+
+    // runs of four elements aligned for one load / store: in the head (dim, pairs) and from row to row
+    const size_t in4 = 4 * isz;
+    bool wide = a->head_dim % 8 == 0 && (inter || p.pairs % 4 == 0);
+    const int64_t strides[6] = {a->q_stride, a->k_stride, has_v ? a->v_stride : 0, a->q_out_stride, a->k_out_stride, has_v ? a->v_out_stride : 0};
+    for (int64_t s : strides) wide = wide && s % 4 == 0;
+    for (const void *x : ins) wide = wide && aligned(x, in4);
+    for (const void *x : outs) wide = wide && aligned(x, 8);
+    wide = wide && aligned(a->q_gain, 16) && aligned(a->k_gain, 16);
+
+    hipStream_t st = (hipStream_t)stream;
+    const bool h = a->out_type == SPTMM_X_F16;
+    switch (a->in_type) {
+    case SPTMM_X_F16: h ? launch_in_out<SPTMM_X_F16, SPTMM_X_F16>(p, inter, wide, blocks, st) : launch_in_out<SPTMM_X_F16, SPTMM_X_BF16>(p, inter, wide, blocks, st); break;
+    case SPTMM_X_BF16: h ? launch_in_out<SPTMM_X_BF16, SPTMM_X_F16>(p, inter, wide, blocks, st) : launch_in_out<SPTMM_X_BF16, SPTMM_X_BF16>(p, inter, wide, blocks, st); break;
+    default: h ? launch_in_out<SPTMM_X_F32, SPTMM_X_F16>(p, inter, wide, blocks, st) : launch_in_out<SPTMM_X_F32, SPTMM_X_BF16>(p, inter, wide, blocks, st); break;
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? SPTMM_OK : fail(SPTMM_ERR_HIP, "heads_kernel launch: %s (%d)", hipGetErrorString(e), (int)e);
+}

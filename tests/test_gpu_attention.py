@@ -1,0 +1,259 @@
+"""GPU: sptmm_attention against the definition in 64 bits (tests/operators64.py holds it and the error bounds)."""
+import numpy as np
+import pytest
+
+import operators64 as op
+import sptmm_amd as sp
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    return sp.device_init(0)
+
+
+class Call:
+    """One attention call: inputs from a seed, strides and gaps as asked, buffers on the device."""
+
+    def __init__(self, seed, nq, nk, heads, dim, t, packed=False, tail=0, gap=5, pad=0, max_q=None, max_kv=None, scale=None, edit=None, sharp=1.5):
+        r = np.random.default_rng(seed)
+        hq, hkv = heads
+        self.t, self.dim, self.hq, self.hkv = t, dim, hq, hkv
+        self.q_start = np.concatenate([[0], np.cumsum(nq)]).astype(np.int32)
+        self.kv_len = np.asarray(nk, np.int32)
+        self.kv_start = self.q_start[:-1].copy() if packed else np.concatenate([[0], np.cumsum(np.asarray(nk) + gap)])[:-1].astype(np.int32)
+        self.rows = max(1, int((self.kv_start + self.kv_len).max()) + (0 if packed else gap))
+        self.total = int(self.q_start[-1]) + tail
+        self.scale = scale or op.softmax_scale(dim)
+        q, k, v = r.standard_normal((self.total, hq, dim)) * sharp, r.standard_normal((self.rows, hkv, dim)), r.standard_normal((self.rows, hkv, dim))
+        if edit:
+            edit(self, q, k, v)
+        self.q, self.k, self.v = (op.narrow(x, t)[1] for x in (q, k, v))
+        wide = [np.full((len(x), x.shape[1] * dim + pad), np.nan, np.float32) for x in (q, k, v)]  # what lies between rows is never read
+        for w, x in zip(wide, (q, k, v)):
+            w[:, : x.shape[1] * dim] = x.reshape(len(x), -1)
+        self.bufs = [sp.DeviceBuffer.from_numpy(op.narrow(w, t)[0]) for w in wide]
+        self.out_pad = pad
+        self.before, _ = op.narrow(r.standard_normal((self.total, hq * dim + self.out_pad)), t)
+        self.out = sp.DeviceBuffer.from_numpy(self.before)
+        ints = [sp.DeviceBuffer.from_numpy(x) for x in (self.q_start, self.kv_start, self.kv_len)]
+        self.bufs += ints
+        self.args = sp.AttentionArgs(q=self.bufs[0], k=self.bufs[1], v=self.bufs[2], out=self.out, q_stride=hq * dim + pad, k_stride=hkv * dim + pad, v_stride=hkv * dim + pad,
+                                     out_stride=hq * dim + self.out_pad, kv_rows=self.rows, q_start=ints[0], kv_start=None if packed else ints[1],
+                                     kv_len=None if packed else ints[2], batch=len(nq), total_q=self.total, max_q=max(nq) if max_q is None else max_q,
+                                     max_kv=max(nk) if max_kv is None else max_kv, q_heads=hq, kv_heads=hkv, head_dim=dim, type=op.CODE[t], scale=self.scale)
+
+    def run(self, stream=None):
+        n = sp.attention_workspace_bytes(self.args)
+        self.ws_bytes = n
+        self.ws = sp.DeviceBuffer(n + 256)
+        self.ws.fill(0xFF)  # NaN everywhere: nothing may be read that was not written
+        sp.attention(self.args, self.ws, n, stream)
+        sp.device_sync()
+        assert (self.ws.to_numpy(np.uint8, n + 256)[n:] == 0xFF).all()
+        self.got = self.out.to_numpy(op.buffer_type(self.t), self.before.shape)
+        return self
+
+    def check(self):
+        want = op.attention(self.q, self.k, self.v, self.q_start, self.kv_start, self.kv_len, self.scale, self.t)
+        got = op.widen(self.got, self.t)
+        for row in range(self.total):
+            mine = got[row, : self.hq * self.dim].reshape(self.hq, self.dim)
+            if row not in want:
+                assert (self.got[row].view(np.uint16) == self.before[row].view(np.uint16)).all(), "row %d behind the last sequence was written" % row
+                continue
+            o, e = want[row]
+            fine = np.isfinite(o)
+            assert (np.isnan(mine) == np.isnan(o)).all(), ("NaN", row)
+            assert (mine[~fine & ~np.isnan(o)] == o[~fine & ~np.isnan(o)]).all(), ("Inf", row)
+            off = np.abs(mine - o)[fine]
+            assert (off <= e[fine]).all(), (row, float((off / e[fine]).max()))
+            if self.out_pad:
+                assert (self.got[row, self.hq * self.dim:].view(np.uint16) == self.before[row, self.hq * self.dim:].view(np.uint16)).all()
+        return self
+
+    def free(self):
+        for b in self.bufs + [self.out, self.ws]:
+            b.free()
+
+
+def one(*a, **k):
+    print("attention", a, {x: y for x, y in k.items() if x != "edit"}, flush=True)
+    c = Call(*a, **k).run()
+    c.check().free()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [8, 64, 72, 80, 128, 136, 256])
+def test_prompts_of_every_width(dim, t):
+    one(1, [1, 33, 0, 130, 7], [1, 33, 0, 130, 7], (4, 2), dim, t, packed=True)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("heads", [(1, 1), (5, 5), (6, 2), (20, 5), (12, 1), (40, 1)])
+def test_heads_per_group(heads, t):
+    one(2, [70, 3], [70, 3], heads, 64, t, packed=True)
+    one(3, [1, 1, 1], [70, 3, 129], heads, 64, t)
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200, 257])
+def test_prompt_lengths(n):
+    one(4, [n], [n], (2, 1), 128, "bf16", packed=True)
+
+
+@pytest.mark.parametrize("m", [0, 1, 31, 32, 33, 64, 127, 128, 129, 255, 256, 257, 1000])
+def test_one_token_against_a_cache(m):
+    one(5, [1], [m], (20, 5), 128, "f16")
+    one(6, [1, 1], [m, 3], (8, 8), 64, "bf16", tail=2)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_ragged_decode_batch_with_empty_caches_and_a_long_one(t):
+    nk = [0, 1, 2, 700, 0, 33, 5000, 128, 127]
+    one(7, [1] * len(nk), nk, (20, 5), 128, t, tail=3)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_chunks_of_prompts_against_longer_and_shorter_caches(dim):
+    # the second sequence's cache is shorter than its chunk (its first rows see nothing), the third's is empty
+    one(8, [40, 50, 9, 1, 100], [500, 20, 0, 77, 1300], (4, 2), dim, "bf16", tail=1)
+    one(9, [3, 5, 0, 2], [300, 4, 10, 2], (8, 2), dim, "f16")
+
+
+def test_rows_strides_and_gaps():
+    one(10, [5, 60], [40, 77], (4, 2), 64, "f16", pad=8, tail=4)
+    one(11, [1, 1], [400, 77], (4, 2), 128, "bf16", pad=24, tail=4)
+
+
+def test_many_sequences():
+    r = np.random.default_rng(0)
+    nk = [int(x) for x in r.integers(0, 40, 150)]
+    one(12, [1] * 150, nk, (4, 4), 64, "f16")
+    one(13, nk, nk, (2, 1), 64, "bf16", packed=True)
+
+
+@pytest.mark.parametrize("max_q,max_kv", [(0, 0), (1, 1), (1, 100000), (100000, 1), (3, 600), (1 << 30, 1 << 30)])
+def test_results_do_not_depend_on_the_hints_being_right(max_q, max_kv):
+    one(14, [1, 40, 3, 129], [900, 700, 3, 129], (4, 2), 128, "bf16", max_q=max_q, max_kv=max_kv)
+
+
+@pytest.mark.parametrize("scale", [1e-6, 0.01, 3.0])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_flat_and_sharp_scores(scale, t):
+    one(15, [1, 90], [600, 90], (4, 2), 64, t, scale=scale)
+
+
+def test_scores_that_climb_and_fall_along_the_keys():
+    def edit(c, q, k, v):
+        k[:] = k * 0.1 + np.linspace(-3, 3, len(k))[:, None, None]
+        q[0::2] = np.abs(q[0::2])
+        q[1::2] = -np.abs(q[1::2])
+    one(16, [2, 70], [2000, 400], (4, 2), 64, "f16", edit=edit)
+    one(17, [1, 1], [3000, 2000], (4, 2), 128, "bf16", edit=edit)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan])
+def test_what_is_not_finite_reaches_the_rows_that_see_it_only(what, t):
+    # rows behind the caches and between them
+    def outside(c, q, k, v):
+        live = np.zeros(len(k), bool)
+        for s, n in zip(c.kv_start, c.kv_len):
+            live[s:s + n] = True
+        k[~live], v[~live] = what, what
+    one(18, [1, 40, 1], [33, 40, 300], (4, 2), 64, t, edit=outside)
+
+    # a value in the middle of a prompt: rows before it are as if it were not there
+    def inside(c, q, k, v):
+        v[37, 0, 5] = what
+        v[150, 1, 63] = what
+    one(19, [200], [200], (4, 2), 64, t, packed=True, edit=inside)
+    one(20, [150, 4], [180, 70], (4, 2), 128, t, edit=inside)
+    one(21, [2, 5], [38, 152], (4, 2), 64, t, edit=inside)
+
+
+def test_a_key_of_minus_infinity_scores_takes_no_weight():
+    def edit(c, q, k, v):
+        q[:] = np.abs(q) + 0.1
+        k[10:40, 0] = -np.inf
+        k[0, :] = -np.inf
+    one(22, [100], [100], (2, 1), 64, "bf16", packed=True, edit=edit)
+    one(23, [1], [300], (2, 1), 64, "f16", edit=edit)
+
+
+def test_cache_rows_behind_four_gigabytes():
+    """A cache whose last rows lie more than 2^32 bytes and 2^31 elements behind its first, read through a wide row stride."""
+    dim, hkv, stride, n = 64, 1, 1 << 22, 600
+    rows = n
+    big = sp.DeviceBuffer(2 * stride * rows)  # 5 GB; only the rows themselves are written
+    r = np.random.default_rng(3)
+    k, kv64 = op.narrow(r.standard_normal((rows, hkv * dim)), "bf16")
+    host = np.zeros((rows, dim), np.uint16)
+    host[:] = k
+    import ctypes as C
+    for i in range(rows):
+        rc = sp.lib().sptmm_memcpy_h2d(C.c_void_p(big.ptr.value + 2 * stride * i), host[i].ctypes.data_as(C.c_void_p), C.c_size_t(2 * dim))
+        assert rc == 0
+    q, q64 = op.narrow(r.standard_normal((2, 2 * dim)), "bf16")
+    qb, out = sp.DeviceBuffer.from_numpy(q), sp.DeviceBuffer(2 * q.size)
+    ints = [sp.DeviceBuffer.from_numpy(np.array(x, np.int32)) for x in ([0, 1, 2], [0, 530], [600, 70])]
+    a = sp.AttentionArgs(q=qb, k=big, v=big, out=out, q_stride=2 * dim, k_stride=stride, v_stride=stride, out_stride=2 * dim, kv_rows=rows, q_start=ints[0], kv_start=ints[1],
+                         kv_len=ints[2], batch=2, total_q=2, max_q=1, max_kv=600, q_heads=2, kv_heads=1, head_dim=dim, type=2, scale=0.125)
+    for max_q in (1, 200):  # both forms
+        print("long cache, max_q", max_q, flush=True)
+        a.max_q = max_q
+        n_ws = sp.attention_workspace_bytes(a)
+        ws = sp.DeviceBuffer(n_ws + 16)
+        sp.attention(a, ws, n_ws)
+        sp.device_sync()
+        got = op.widen(out.to_numpy(np.uint16, (2, 2, dim)), "bf16")
+        want = op.attention(q64.reshape(2, 2, dim), kv64.reshape(rows, 1, dim), kv64.reshape(rows, 1, dim), [0, 1, 2], [0, 530], [600, 70], 0.125, "bf16")
+        for row in (0, 1):
+            assert (np.abs(got[row] - want[row][0]) <= want[row][1]).all()
+        ws.free()
+    for b in [big, qb, out] + ints:
+        b.free()
+
+
+def test_a_captured_call_follows_its_buffers():
+    """Three replays with new queries, keys and lengths in the captured buffers, eager work between them."""
+    st = sp.Stream()
+    c = Call(30, [1, 1, 1], [900, 40, 0], (20, 5), 128, "bf16", max_kv=2000, gap=600)
+    n = sp.attention_workspace_bytes(c.args)
+    c.ws = sp.DeviceBuffer(n + 256)
+    with sp.Graph(st) as g:
+        sp.attention(c.args, c.ws, n, st)
+    r = np.random.default_rng(5)
+    for rep in range(3):
+        print("replay", rep, flush=True)
+        qb, c.q = op.narrow(r.standard_normal(c.q.shape), "bf16")
+        kb, c.k = op.narrow(r.standard_normal(c.k.shape), "bf16")
+        c.kv_len = np.array([1500 - 300 * rep, 41 + rep, rep], np.int32)
+        c.bufs[0].upload(qb)
+        c.bufs[1].upload(kb)
+        c.bufs[5].upload(c.kv_len)
+        g.launch(st)
+        st.sync()
+        first = c.out.to_numpy(np.uint16, c.before.shape)
+        c.got = first
+        c.check()
+        c.out.upload(c.before)
+        sp.attention(c.args, c.ws, n, st)  # the program's own eager work
+        st.sync()
+        assert (c.out.to_numpy(np.uint16, c.before.shape) == first).all()
+    g.destroy()
+    c.free()
+    st.destroy()
+
+
+def test_lengths_that_lead_out_of_the_buffers_are_cut():
+    """The arrays on the device are data: whatever they hold, nothing outside the buffers is read or written (the rows' values are
+    not specified then; the call returns and the device goes on working)."""
+    c = Call(31, [4, 4, 4], [20, 20, 20], (4, 2), 64, "f16", tail=2)
+    c.bufs[3].upload(np.array([0, 9, 3, 1 << 30], np.int32))
+    c.bufs[4].upload(np.array([-5, 1 << 30, 40], np.int32))
+    c.bufs[5].upload(np.array([1 << 30, 10, 1 << 30], np.int32))
+    c.run()
+    c.free()
+    one(32, [4, 4], [20, 20], (4, 2), 64, "f16")
