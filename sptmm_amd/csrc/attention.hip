@@ -157,6 +157,7 @@ template <int DP, int KT, int WAVES> struct Loader {
 
 // ------------------------------------------------------------------------------------------------ one wavefront's rows
 template <int T, int DP, int KT> struct Rows {
+    enum { CLEAN, EDGE };
     static constexpr int KS = DP / 16, DS = DP / 32, KB = KT / 32;
     u16x8 qf[KS];
     f32x16 o[DS];
@@ -188,16 +189,19 @@ template <int T, int DP, int KT> struct Rows {
         for (int d = 0; d < DS; ++d) v_at[d] = vr * DP * 2 + (((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swizzle_v<DP>(vr)) << 4) + (lane & 1) * 8;
     }
 
-    // values of V that are not finite, anywhere in the tile
-    __device__ __forceinline__ bool not_finite(const char *v) const
+    // A row's p is zero at keys it does not see, and zero times an infinity is not zero.  Where some row of this wavefront does not
+    // see every key that the tile holds (those before `end`; lo: the smallest last key of the rows), a tile of V with a value
+    // that is not finite is added key by key, to the rows that see the key.
+    __device__ __forceinline__ bool polluted(const char *v, int j0, int end, int lo) const
     {
+        if (min(j0 + KT, end) - 1 <= lo) return false;
         const int lane = threadIdx.x & 63;
         bool bad = false;
         constexpr unsigned E = T == SPTMM_X_F16 ? 0x7c00u : 0x7f80u;
         for (int i = lane; i < KT * DP / 8; i += 64) {
             const u32x4 w = *reinterpret_cast<const u32x4 *>(v + i * 16);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bad = bad || (w[j] & E) == E || ((w[j] >> 16) & E) == E;
+            for (int j = 0; j < 4; ++j) bad = bad || (w[j] & E) == E || (w[j] & E << 16) == E << 16;
         }
         return __ballot(bad) != 0;
     }
@@ -211,8 +215,8 @@ template <int T, int DP, int KT> struct Rows {
         return __builtin_bit_cast(u16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 
-    // the tile of keys from j0 on, of which those before `end` are there; lo: the smallest last key of this wavefront's rows
-    __device__ __forceinline__ void step(const AttnParams &p, const char *k, const char *v, int j0, int end, int lo)
+    // One tile of keys, from j0 on.  CLEAN: every row of this wavefront sees all of it; EDGE: some do not.  bad: see `polluted`.
+    template <int KIND> __device__ __forceinline__ void step(const AttnParams &p, const char *k, const char *v, int j0, bool bad = false)
     {
         const int half = (threadIdx.x & 63) >> 5;
         f32x16 s[KB];
@@ -225,12 +229,12 @@ template <int T, int DP, int KT> struct Rows {
 #pragma unroll
             for (int b = 0; b < KB; ++b)
                 s[b] = mfma<T>(*reinterpret_cast<const u16x8 *>(k + (k_at ^ (ks << 5)) + b * 32 * DP * 2), qf[ks], s[b]);
-        const bool edge = j0 + KT - 1 > lo;
-        if (edge) {
+        if (KIND != CLEAN) {
+            const int last = lim - j0 - 4 * half;
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[b][e] = j0 + b * 32 + 8 * (e >> 2) + 4 * half + (e & 3) <= lim ? s[b][e] : -INFINITY;
+                for (int e = 0; e < 16; ++e) s[b][e] = b * 32 + 8 * (e >> 2) + (e & 3) <= last ? s[b][e] : -INFINITY;
         }
         float mx = s[0][0];
 #pragma unroll
@@ -258,33 +262,30 @@ template <int T, int DP, int KT> struct Rows {
                 sum += x;
                 pf[2 * b + (e >> 3)][e & 7] = narrow<T>(x);
             }
-        // A row's p is zero at keys it does not see, and zero times an infinity is not: where some row of this wavefront does not
-        // see every key of the tile, values that are not finite are added key by key, for the rows that see the key.
-        if (edge && min(j0 + KT, end) - 1 > lo && not_finite(v)) {
+        if (KIND == EDGE && bad) {
+            const f32x16 zero = {0.f};
 #pragma unroll
             for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll 1
-                for (int x = 0; x < 16; ++x) {
-                    const int e = x & 7;  // element x % 8 of the lower (x < 8) or upper lanes' eight keys
-                    const int key = j0 + 16 * t + (e < 4 ? e : e + 4) + 4 * (x >> 3);
-                    const bool mine = half == x >> 3;
+                for (int x = 0; x < 16; ++x) {  // element x % 8 of the lower (x < 8) or the upper lanes' eight keys of step t
+                    const int e = x & 7, key = j0 + 16 * t + (e < 4 ? e : e + 4) + 4 * (x >> 3);
                     u32x4 only;
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) only[w] = mine && w == e >> 1 ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+                    for (int w = 0; w < 4; ++w) only[w] = half == x >> 3 && w == e >> 1 ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
                     const u16x8 one = __builtin_bit_cast(u16x8, __builtin_bit_cast(u32x4, pf[t]) & only);
 #pragma unroll
                     for (int d = 0; d < DS; ++d) {
-                        const f32x16 n = mfma<T>(__builtin_bit_cast(u16x8, __builtin_bit_cast(u32x4, v_frag(v, d, t)) & only), one, o[d]);
+                        const f32x16 n = mfma<T>(__builtin_bit_cast(u16x8, __builtin_bit_cast(u32x4, v_frag(v, d, t)) & only), one, zero);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[d][i] = key <= lim ? n[i] : o[d][i];
+                        for (int i = 0; i < 16; ++i) o[d][i] += key <= lim ? n[i] : 0.f;
                     }
                 }
-            return;
+        } else {
+#pragma unroll
+            for (int d = 0; d < DS; ++d)
+#pragma unroll
+                for (int t = 0; t < 2 * KB; ++t) o[d] = mfma<T>(v_frag(v, d, t), pf[t], o[d]);
         }
-#pragma unroll
-        for (int d = 0; d < DS; ++d)
-#pragma unroll
-            for (int t = 0; t < 2 * KB; ++t) o[d] = mfma<T>(v_frag(v, d, t), pf[t], o[d]);
     }
 };
 
@@ -329,19 +330,37 @@ template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64
     lv.init(p.v_stride, p.dim, wave, true);
     const u16 *k = p.k + (int64_t)t.k0 * p.k_stride + (int64_t)kv_head * p.dim, *v = p.v + (int64_t)t.k0 * p.v_stride + (int64_t)kv_head * p.dim;
 
-    auto load = [&](int j, char *kl, char *vl) {
+    const int n = begin < end ? (end - begin + KT - 1) / KT : 0;
+    // tiles that every row of the workgroup sees whole, in pairs: the two pairs of buffers alternate by name, so that the compiler
+    // knows which loads a read has to wait for
+    const int clean = max(0, min(t.nk - t.nq + t.row0 / p.group + 1, end) - begin) / KT & ~1;
+    auto load = [&](int i, char *kl, char *vl) {
+        if (i >= n) return;
+        const int j = begin + i * KT;
         lk.issue(k + (int64_t)j * p.k_stride, p.k_stride, p.dim, end - j, kl, wave);
         lv.issue(v + (int64_t)j * p.v_stride, p.v_stride, p.dim, end - j, vl, wave);
     };
-    if (begin < end) load(begin, k_a, v_a);
-    for (int j = begin; j < end; j += 2 * KT) {
+    typedef Rows<T, DP, KT> R;
+    load(0, k_a, v_a);
+    int i = 0;
+    for (; i < clean; i += 2) {
         lds_arrived();
-        if (j + KT < end) load(j + KT, k_b, v_b);
-        if (j <= hi) r.step(p, k_a, v_a, j, end, lo);
-        if (j + KT >= end) break;
+        load(i + 1, k_b, v_b);
+        r.template step<R::CLEAN>(p, k_a, v_a, 0);
         lds_arrived();
-        if (j + 2 * KT < end) load(j + 2 * KT, k_a, v_a);
-        if (j + KT <= hi) r.step(p, k_b, v_b, j + KT, end, lo);
+        load(i + 2, k_a, v_a);
+        r.template step<R::CLEAN>(p, k_b, v_b, 0);
+    }
+    for (; i < n; ++i) {
+        int j = begin + i * KT;
+        lds_arrived();
+        load(i + 1, k_b, v_b);
+        if (j <= hi) r.template step<R::EDGE>(p, k_a, v_a, j, r.polluted(v_a, j, end, lo));
+        if (++i >= n) break;
+        j += KT;
+        lds_arrived();
+        load(i + 1, k_a, v_a);
+        if (j <= hi) r.template step<R::EDGE>(p, k_b, v_b, j, r.polluted(v_b, j, end, lo));
     }
     const float sum = halves_sum(r.sum), f = p.splits > 1 ? 1.f : 1.f / sum;
     if (!valid) return;
@@ -384,28 +403,39 @@ template <int T, int DP, int WAVES> __global__ void __launch_bounds__(64 * WAVES
     lk.init(p.k_stride, p.dim, 0, false);
     lv.init(p.v_stride, p.dim, 0, true);
     const u16 *k = p.k + (int64_t)t.k0 * p.k_stride + (int64_t)kv_head * p.dim, *v = p.v + (int64_t)t.k0 * p.v_stride + (int64_t)kv_head * p.dim;
-    auto load = [&](int j, char *kl, char *vl) {
-        lk.issue(k + (int64_t)j * p.k_stride, p.k_stride, p.dim, end - j, kl + wave * ONE, 0);
-        lv.issue(v + (int64_t)j * p.v_stride, p.v_stride, p.dim, end - j, vl + wave * ONE, 0);
-    };
     // this wavefront's tiles: every WAVES-th, one in use while the next is on its way
     constexpr int STRIDE = WAVES * KT;
-    auto wait = [&](bool next) {
-        if (next) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Loader<DP, KT, 1>::PER) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const int j0 = begin + wave * KT, n = j0 < end ? (end - j0 + STRIDE - 1) / STRIDE : 0;
+    const int whole = min(lo + 1, end) - j0, clean = (whole < KT ? 0 : (whole - KT) / STRIDE + 1) & ~1;
+    auto load = [&](int i, char *kl, char *vl) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the tile that this load overwrites are done
+        if (i < n) {
+            const int j = j0 + i * STRIDE;
+            lk.issue(k + (int64_t)j * p.k_stride, p.k_stride, p.dim, end - j, kl + wave * ONE, 0);
+            lv.issue(v + (int64_t)j * p.v_stride, p.v_stride, p.dim, end - j, vl + wave * ONE, 0);
+            if (i) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Loader<DP, KT, 1>::PER) : "memory");  // the tile before this one has landed
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
     };
-    int j = begin + wave * KT;
-    if (j < end) load(j, k_a, v_a);
-    for (; j < end; j += 2 * STRIDE) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (j + STRIDE < end) load(j + STRIDE, k_b, v_b);
-        wait(j + STRIDE < end);
-        r.step(p, k_a + wave * ONE, v_a + wave * ONE, j, end, lo);
-        if (j + STRIDE >= end) break;
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the tile that the next load overwrites are done
-        if (j + 2 * STRIDE < end) load(j + 2 * STRIDE, k_a, v_a);
-        wait(j + 2 * STRIDE < end);
-        r.step(p, k_b + wave * ONE, v_b + wave * ONE, j + STRIDE, end, lo);
+    typedef Rows<T, DP, KT> R;
+    char *const ka = k_a + wave * ONE, *const kb = k_b + wave * ONE, *const va = v_a + wave * ONE, *const vb = v_b + wave * ONE;
+    load(0, k_a, v_a);
+    int i = 0;
+    for (; i < clean; i += 2) {
+        load(i + 1, k_b, v_b);
+        r.template step<R::CLEAN>(p, ka, va, 0);
+        load(i + 2, k_a, v_a);
+        r.template step<R::CLEAN>(p, kb, vb, 0);
+    }
+    for (; i < n; ++i) {
+        int j = j0 + i * STRIDE;
+        load(i + 1, k_b, v_b);
+        r.template step<R::EDGE>(p, ka, va, j, r.polluted(va, j, end, lo));
+        if (++i >= n) break;
+        j += STRIDE;
+        load(i + 1, k_a, v_a);
+        r.template step<R::EDGE>(p, kb, vb, j, r.polluted(vb, j, end, lo));
     }
     // the wavefronts' sums, brought to one maximum and added in wavefront order; a wavefront's part lies where its tiles lay
     const float sum = halves_sum(r.sum);
@@ -477,21 +507,48 @@ template <int T> __global__ void __launch_bounds__(256) attention_join_kernel(co
     nk = k0 < 0 || k0 >= p.kv_rows ? 0 : min(max(nk, (int64_t)0), p.kv_rows - k0);
     const int seen = (int)nk - (q1 - q0) + (query - q0) + 1;
     const int n = seen <= 0 ? 0 : min(p.splits, (seen + p.chunk - 1) / p.chunk);
-    float top = -INFINITY;
-    for (int s = 0; s < n; ++s) top = fmaxf(top, p.part_ml[s * all + row].x);
-    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < n; ++s) {
-        const float2 ml = p.part_ml[s * all + row];
-        const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - top) * p.c);
-        sum = fmaf(ml.y, f, sum);
+    // every lane holds the weight of one split (and of those 64, 128 and 192 further)
+    float2 ml[4];
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 64 * i < p.dim) o[i] = fmaf(p.part_o[(s * all + row) * p.dim + lane + 64 * i], f, o[i]);
+    for (int i = 0; i < 4; ++i) {
+        ml[i] = lane + 64 * i < n ? p.part_ml[(lane + 64 * i) * all + row] : float2{-INFINITY, 0.f};
+        top = fmaxf(top, ml[i].x);
     }
-    const float inv = n ? 1.f / sum : 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < p.dim) p.out[(int64_t)query * p.out_stride + (int64_t)head * p.dim + lane + 64 * i] = narrow<T>(n ? o[i] * inv : 0.f);
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    float w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i].x - top) * p.c);
+        sum = fmaf(ml[i].y, w[i], sum);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    // four values a lane, and as many splits side by side as lanes are left
+    const int quads = p.dim / 4, log_l = quads <= 2 ? 1 : 32 - __builtin_clz(quads - 1), sub = lane >> log_l, d4 = lane & ((1 << log_l) - 1), step = 64 >> log_l;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (64 * i >= n) break;
+        for (int s0 = 64 * i; s0 < min(n, 64 * i + 64); s0 += step) {
+            const int s = s0 + sub;
+            const float f = __shfl(w[i], s & 63, 64);
+            if (s < n && d4 < quads) {
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(p.part_o + (s * all + row) * p.dim + 4 * d4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+            }
+        }
+    }
+    for (int l = 1 << log_l; l < 64; l <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], l, 64);
+    const float inv = 1.f / sum;
+    u16x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = narrow<T>(n ? o[e] * inv : 0.f);
+    if (sub == 0 && d4 < quads) *reinterpret_cast<u16x4 *>(p.out + (int64_t)query * p.out_stride + (int64_t)head * p.dim + 4 * d4) = y;
 }
 
 int check(const sptmm_attention_args *a)
