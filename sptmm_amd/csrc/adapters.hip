@@ -88,51 +88,86 @@ __device__ __forceinline__ int next_slot(int slot, unsigned long long &left)
     return s;
 }
 
+// slot of the row that this lane holds (row tile * 16 + lane % 16), -1 where it has none
+__device__ __forceinline__ int slot_of(const AdapterArgs &p, int m)
+{
+    const int s = m < p.M ? p.row_slot[m] : -1;
+    return s >= 0 && s < p.slots ? s : -1;
+}
+
 // ------------------------------------------------------------------------------------------------ h = X A^T
 constexpr int SHRINK_WAVES = 8;
 constexpr int CHUNKS_AT_ONCE = 4;  // chunks of 16 ranks summed in one walk over K (X is read once per walk)
+constexpr int STEPS_AT_ONCE = 4;   // steps of 32 along K whose loads are in flight together
 
-// Workgroup (tile of 16 rows, split of K, ordinal of a distinct slot in the tile): eight wavefronts take every eighth step of the
-// split's range of K, and add their sums through the LDS in wavefront order.  ONE: a workgroup serves one slot of its tile (few
-// rows: slots spread over workgroups); else it walks them all.
+// this wavefront's share of NC chunks' sums over the steps step0, step0 + SHRINK_WAVES, ... below step1
+template <int T, int NC> __device__ __forceinline__ void walk_k(const AdapterArgs &p, const u16 *a, const u16 *x_row, int step0, int step1, f32x4 (&acc)[CHUNKS_AT_ONCE])
+{
+    const int k_lane = 8 * ((threadIdx.x & 63) >> 4);
+    for (int step = step0; step < step1; step += STEPS_AT_ONCE * SHRINK_WAVES) {
+        u16x8 x[STEPS_AT_ONCE], w[STEPS_AT_ONCE][NC];
+#pragma unroll
+        for (int u = 0; u < STEPS_AT_ONCE; ++u) {
+            const int at = min(step + u * SHRINK_WAVES, step1 - 1);
+            x[u] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+            if (32 * at + k_lane < p.K) x[u] = *reinterpret_cast<const u16x8 *>(x_row + 32 * at);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) w[u][c] = *reinterpret_cast<const u16x8 *>(a + ((int64_t)c * p.k_steps + at) * 512);
+        }
+#pragma unroll
+        for (int u = 0; u < STEPS_AT_ONCE; ++u)
+            if (step + u * SHRINK_WAVES < step1)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) acc[c] = mfma16<T>(w[u][c], x[u], acc[c]);
+    }
+}
+
+// chunks c0 .. c0 + nc - 1 of slot s, summed over a range of K by the workgroup's eight wavefronts: afterwards wavefront w < nc
+// holds chunk c0 + w of all 16 rows.  The wavefronts' shares are added through the LDS in wavefront order.
+template <int T> __device__ __forceinline__ f32x4 shrink(const AdapterArgs &p, f32x4 (&sums)[SHRINK_WAVES][CHUNKS_AT_ONCE][64], int s, int c0, int nc, const u16 *x_row, int step0, int step1)
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    f32x4 acc[CHUNKS_AT_ONCE];
+#pragma unroll
+    for (int c = 0; c < CHUNKS_AT_ONCE; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const u16 *a = p.A + ((int64_t)s * p.max_chunks + c0) * p.k_steps * 512 + lane * 8;
+    switch (nc) {
+    case 1: walk_k<T, 1>(p, a, x_row, step0 + wave, step1, acc); break;
+    case 2: walk_k<T, 2>(p, a, x_row, step0 + wave, step1, acc); break;
+    case 3: walk_k<T, 3>(p, a, x_row, step0 + wave, step1, acc); break;
+    default: walk_k<T, 4>(p, a, x_row, step0 + wave, step1, acc); break;
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS_AT_ONCE; ++c)
+        if (c < nc) sums[wave][c][lane] = acc[c];
+    __syncthreads();
+    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    if (wave < nc) {
+        t = sums[0][wave][lane];
+#pragma unroll
+        for (int w = 1; w < SHRINK_WAVES; ++w) t += sums[w][wave][lane];
+    }
+    return t;
+}
+
+// Workgroup (tile of 16 rows, split of K, ordinal of a distinct slot in the tile).  ONE: it serves one slot of its tile (few rows:
+// slots spread over workgroups); else it walks them all.
 template <int T, bool ONE> __global__ void __launch_bounds__(SHRINK_WAVES * 64) adapters_shrink_kernel(const AdapterArgs p)
 {
     __shared__ __attribute__((aligned(16))) f32x4 sums[SHRINK_WAVES][CHUNKS_AT_ONCE][64];
     const int tile = blockIdx.x, split = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int m = tile * 16 + (lane & 15);
-    int slot = m < p.M ? p.row_slot[m] : -1;
-    if (slot < 0 || slot >= p.slots) slot = -1;
+    const int m = tile * 16 + (lane & 15), slot = slot_of(p, m);
     unsigned long long left = __ballot(slot >= 0) & 0xffff;
     if (ONE)
         for (int o = blockIdx.z; o > 0 && left; --o) next_slot(slot, left);
-    // this workgroup's steps of K
     const int per = (p.k_steps + p.splits - 1) / p.splits, step0 = split * per, step1 = min(p.k_steps, step0 + per);
     const u16 *x_row = p.X + (int64_t)min(m, p.M - 1) * p.K + 8 * (lane >> 4);
     while (left) {
         const int s = next_slot(slot, left), chunks = p.chunks[s];
         for (int c0 = 0; c0 < chunks; c0 += CHUNKS_AT_ONCE) {
             const int nc = min(CHUNKS_AT_ONCE, chunks - c0);
-            f32x4 acc[CHUNKS_AT_ONCE];
-#pragma unroll
-            for (int c = 0; c < CHUNKS_AT_ONCE; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-            const u16 *a = p.A + (((int64_t)s * p.max_chunks + c0) * p.k_steps) * 512 + lane * 8;
-#pragma unroll 4
-            for (int step = step0 + wave; step < step1; step += SHRINK_WAVES) {
-                u16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (32 * step + 8 * (lane >> 4) < p.K) x = *reinterpret_cast<const u16x8 *>(x_row + 32 * step);
-#pragma unroll
-                for (int c = 0; c < CHUNKS_AT_ONCE; ++c)
-                    if (c < nc) acc[c] = mfma16<T>(*reinterpret_cast<const u16x8 *>(a + ((int64_t)c * p.k_steps + step) * 512), x, acc[c]);
-            }
-#pragma unroll
-            for (int c = 0; c < CHUNKS_AT_ONCE; ++c)
-                if (c < nc) sums[wave][c][lane] = acc[c];
-            __syncthreads();
-            if (wave < nc) {
-                f32x4 t = sums[0][wave][lane];
-                for (int w = 1; w < SHRINK_WAVES; ++w) t += sums[w][wave][lane];
-                if (slot == s) reinterpret_cast<f32x4 *>(p.h)[(((int64_t)split * p.tiles + tile) * p.max_chunks + c0 + wave) * 64 + lane] = t;
-            }
+            const f32x4 t = shrink<T>(p, sums, s, c0, nc, x_row, step0, step1);
+            if (wave < nc && slot == s) reinterpret_cast<f32x4 *>(p.h)[(((int64_t)split * p.tiles + tile) * p.max_chunks + c0 + wave) * 64 + lane] = t;
             __syncthreads();
         }
         if (ONE) break;
@@ -140,24 +175,41 @@ template <int T, bool ONE> __global__ void __launch_bounds__(SHRINK_WAVES * 64) 
 }
 
 // ------------------------------------------------------------------------------------------------ Y = base + scale * h B^T
-// A wavefront takes 16 * RT rows and 32 columns.  ONE: only the rows of one distinct slot of its tile (and, the first of them,
-// the rows without a slot); else all slots of its rows.
+// 16 rows x 32 columns of one chunk of 16 ranks, on the 32-bit matrix instruction; rows that do not use the slot keep y
+template <int T> __device__ __forceinline__ void add_chunk(u16x8 b, f32x4 h, bool mine, f32x4 &y0, f32x4 &y1)
+{
+    f32x4 n0 = y0, n1 = y1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        n0 = __builtin_amdgcn_mfma_f32_16x16x4f32(widen<T>(b[e]), h[e], n0, 0, 0, 0);
+        n1 = __builtin_amdgcn_mfma_f32_16x16x4f32(widen<T>(b[4 + e]), h[e], n1, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y0[e] = mine ? n0[e] : y0[e], y1[e] = mine ? n1[e] : y1[e];
+}
+// the operand of column pair `pair`, chunk c of slot s (`chunks` chunks in use)
+__device__ __forceinline__ u16x8 load_b(const AdapterArgs &p, int s, int pair, int chunks, int c)
+{
+    return *reinterpret_cast<const u16x8 *>(p.B + ((int64_t)s * p.n_pairs * p.max_chunks + (int64_t)pair * chunks + c) * 512 + (threadIdx.x & 63) * 8);
+}
+
+// A workgroup takes 16 * RT rows and its four wavefronts 32 columns each.  Every row's h (its own slot's) is first brought into the
+// LDS, scaled and with the splits' partial sums added in their order; then the distinct slots are walked.
+// ONE (RT = 1): only the rows of one distinct slot of the tile (and, the first of them, the rows without a slot).
 template <int T, int RT, bool ONE> __global__ void __launch_bounds__(256) adapters_expand_kernel(const AdapterArgs p)
 {
-    const int lane = threadIdx.x & 63, pair = blockIdx.y * 4 + (threadIdx.x >> 6), tile0 = blockIdx.x * RT;
-    if (pair >= p.n_pairs) return;
-    int slot[RT];
+    extern __shared__ __attribute__((aligned(16))) f32x4 h_lds[];  // [RT][max_chunks][64]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int groups = (p.n_pairs + 3) / 4, tile0 = (int)(blockIdx.x / groups) * RT, pair = (int)(blockIdx.x % groups) * 4 + wave;
+    int slot[RT], chunks_of[RT];
     bool write[RT];
-    unsigned long long left[RT], any = 0;
+    unsigned long long left[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int m = (tile0 + t) * 16 + (lane & 15);
-        int s = m < p.M ? p.row_slot[m] : -1;
-        if (s < 0 || s >= p.slots) s = -1;
-        slot[t] = s;
-        left[t] = __ballot(s >= 0) & 0xffff;
+        slot[t] = slot_of(p, m);
+        left[t] = __ballot(slot[t] >= 0) & 0xffff;
         write[t] = m < p.M;
-        any |= left[t];
     }
     if (ONE) {
         for (int o = blockIdx.z; o > 0 && left[0]; --o) next_slot(slot[0], left[0]);
@@ -167,7 +219,7 @@ template <int T, int RT, bool ONE> __global__ void __launch_bounds__(256) adapte
         left[0] &= __ballot(slot[0] == mine);
     }
     const int n0 = pair * 32 + 4 * (lane >> 4);
-    const bool second = pair * 32 + 16 < p.N;  // (an odd number of 16-column groups: the last pair has one)
+    const bool first = pair < p.n_pairs, second = pair * 32 + 16 < p.N;  // (an odd number of 16-column groups: the last pair has one)
     f32x4 acc[RT][2];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -175,9 +227,31 @@ template <int T, int RT, bool ONE> __global__ void __launch_bounds__(256) adapte
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             acc[t][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (p.base && write[t] && (g == 0 || second)) acc[t][g] = *reinterpret_cast<const f32x4 *>(p.base + at + 16 * g);
+            if (p.base && write[t] && (g ? second : first)) acc[t][g] = *reinterpret_cast<const f32x4 *>(p.base + at + 16 * g);
         }
     }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        chunks_of[t] = slot[t] >= 0 && write[t] ? p.chunks[slot[t]] : 0;
+        const float scale = chunks_of[t] ? p.scale[slot[t]] : 0.f;
+        for (int c = wave; c < p.max_chunks; c += 4) {
+            if (!__ballot(c < chunks_of[t])) break;
+            if (c < chunks_of[t]) {
+                const f32x4 *hp = reinterpret_cast<const f32x4 *>(p.h) + ((int64_t)(tile0 + t) * p.max_chunks + c) * 64 + lane;
+                const int64_t next = (int64_t)p.tiles * p.max_chunks * 64;
+                f32x4 h = hp[0];
+                int k = 1;
+                for (; k + 4 <= p.splits; k += 4) {
+                    const f32x4 a = hp[k * next], b = hp[(k + 1) * next], c4 = hp[(k + 2) * next], d = hp[(k + 3) * next];
+                    h += a, h += b, h += c4, h += d;
+                }
+                for (; k < p.splits; ++k) h += hp[k * next];
+                h_lds[(t * p.max_chunks + c) * 64 + lane] = h * scale;
+            }
+        }
+    }
+    __syncthreads();
+    if (!first) return;
 #pragma unroll
     for (int t0 = 0; t0 < RT; ++t0) {
         while (left[t0]) {  // distinct slots of all the rows: those of a later tile are served with the first tile that has them
@@ -189,30 +263,13 @@ template <int T, int RT, bool ONE> __global__ void __launch_bounds__(256) adapte
                 has[t] = t >= t0 && b;
                 if (t > t0) left[t] &= ~b;
             }
-            const float scale = p.scale[s];
+            u16x8 b = load_b(p, s, pair, chunks, 0);
             for (int c = 0; c < chunks; ++c) {
-                const u16x8 b = *reinterpret_cast<const u16x8 *>(p.B + ((int64_t)s * p.n_pairs * p.max_chunks + (int64_t)pair * chunks + c) * 512 + lane * 8);
-                float bw[8];
+                const u16x8 now = b;
+                if (c + 1 < chunks) b = load_b(p, s, pair, chunks, c + 1);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) bw[e] = widen<T>(b[e]);
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    if (!has[t]) continue;
-                    const f32x4 *hp = reinterpret_cast<const f32x4 *>(p.h) + ((int64_t)(tile0 + t) * p.max_chunks + c) * 64 + lane;
-                    f32x4 h = {0.f, 0.f, 0.f, 0.f};
-                    if (slot[t] == s) {
-                        h = hp[0];
-                        for (int k = 1; k < p.splits; ++k) h += hp[(int64_t)k * p.tiles * p.max_chunks * 64];
-                        h *= scale;
-                    }
-                    f32x4 y0 = acc[t][0], y1 = acc[t][1];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        y0 = __builtin_amdgcn_mfma_f32_16x16x4f32(bw[e], h[e], y0, 0, 0, 0);
-                        y1 = __builtin_amdgcn_mfma_f32_16x16x4f32(bw[4 + e], h[e], y1, 0, 0, 0);
-                    }
-                    if (slot[t] == s) acc[t][0] = y0, acc[t][1] = y1;
-                }
+                for (int t = 0; t < RT; ++t)
+                    if (has[t]) add_chunk<T>(now, h_lds[(t * p.max_chunks + c) * 64 + lane], slot[t] == s, acc[t][0], acc[t][1]);
             }
         }
     }
@@ -226,13 +283,55 @@ template <int T, int RT, bool ONE> __global__ void __launch_bounds__(256) adapte
     }
 }
 
+// ------------------------------------------------------------------------------------------------ both products in one launch
+// For a row or a few: workgroup (256 columns, tile, ordinal of a distinct slot) computes its rows' h whole -- every workgroup of a
+// slot reads all of A, which costs less than a second launch while A is small -- and multiplies it by its columns of B.
+template <int T> __global__ void __launch_bounds__(SHRINK_WAVES * 64) adapters_fused_kernel(const AdapterArgs p)
+{
+    __shared__ __attribute__((aligned(16))) f32x4 sums[SHRINK_WAVES][CHUNKS_AT_ONCE][64], h_lds[CHUNKS_AT_ONCE][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = blockIdx.x * SHRINK_WAVES + wave;
+    const int m = blockIdx.y * 16 + (lane & 15), slot = slot_of(p, m);
+    unsigned long long left = __ballot(slot >= 0) & 0xffff;
+    for (int o = blockIdx.z; o > 0 && left; --o) next_slot(slot, left);
+    if (!left && blockIdx.z) return;
+    const int s = left ? __builtin_amdgcn_readlane(slot, __builtin_ctzll(left)) : -2, chunks = left ? p.chunks[s] : 0;
+    const bool write = m < p.M && (slot == s || (blockIdx.z == 0 && slot < 0));
+    const int n0 = pair * 32 + 4 * (lane >> 4);
+    const bool first = pair < p.n_pairs, second = pair * 32 + 16 < p.N;
+    const int64_t at = (int64_t)m * p.N + n0;
+    f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    if (p.base && write && first) acc[0] = *reinterpret_cast<const f32x4 *>(p.base + at);
+    if (p.base && write && second) acc[1] = *reinterpret_cast<const f32x4 *>(p.base + at + 16);
+    const float scale = chunks ? p.scale[s] : 0.f;
+    const u16 *x_row = p.X + (int64_t)min(m, p.M - 1) * p.K + 8 * (lane >> 4);
+    for (int c0 = 0; c0 < chunks; c0 += CHUNKS_AT_ONCE) {
+        const int nc = min(CHUNKS_AT_ONCE, chunks - c0);
+        u16x8 b[CHUNKS_AT_ONCE];
+        if (first)
+#pragma unroll
+            for (int c = 0; c < CHUNKS_AT_ONCE; ++c) b[c] = load_b(p, s, pair, chunks, min(c0 + c, chunks - 1));
+        const f32x4 t = shrink<T>(p, sums, s, c0, nc, x_row, 0, p.k_steps);
+        if (wave < nc) h_lds[wave][lane] = t * scale;
+        __syncthreads();
+        if (first)
+#pragma unroll
+            for (int c = 0; c < CHUNKS_AT_ONCE; ++c)
+                if (c < nc) add_chunk<T>(b[c], h_lds[c][lane], slot == s, acc[0], acc[1]);
+    }
+    if (write && first) *reinterpret_cast<f32x4 *>(p.Y + at) = acc[0];
+    if (write && second) *reinterpret_cast<f32x4 *>(p.Y + at + 16) = acc[1];
+}
+
 int hip_fail(hipError_t e, const char *what) { return fail(SPTMM_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e); }
 
 // Up to this many rows the distinct slots of a tile go to workgroups of their own (decode: every row may have another one, and a
 // workgroup that walks sixteen waits for sixteen chains of loads); beyond it, prompts, a tile rarely has more than two.
 constexpr int SPREAD_ROWS = 128;
+// Up to this much of A (KiB of the largest slot), and one tile of rows, both products run in one launch.
+constexpr int FUSED_A_KIB = 160;
 
 int ordinals(int M) { return M <= SPREAD_ROWS ? (M < 16 ? M : 16) : 1; }
+bool fused(const sptmm_adapters *a, int M) { return M <= 16 && a->max_chunks * a->k_steps <= FUSED_A_KIB; }
 
 // splits of K over workgroups: enough of them to fill the chip, each wavefront with two steps of 32 at least
 int splits_of(const sptmm_adapters *a, int M)
@@ -244,7 +343,7 @@ int splits_of(const sptmm_adapters *a, int M)
 
 size_t need(const sptmm_adapters *a, int M)
 {
-    return (size_t)splits_of(a, M) * ((M + 15) / 16) * a->max_chunks * 64 * 16;
+    return fused(a, M) ? 0 : (size_t)splits_of(a, M) * ((M + 15) / 16) * a->max_chunks * 64 * 16;
 }
 
 int check_device(const sptmm_adapters *a)
@@ -256,14 +355,24 @@ int check_device(const sptmm_adapters *a)
     return SPTMM_OK;
 }
 
-template <int T> void launch_apply(const AdapterArgs &p, int ord, hipStream_t st)
+template <int T> void launch_apply(const AdapterArgs &p, bool one_launch, int ord, hipStream_t st)
 {
-    if (ord > 1 || p.M <= SPREAD_ROWS) {
+    if (one_launch) {
+        hipLaunchKernelGGL((adapters_fused_kernel<T>), dim3((p.n_pairs + SHRINK_WAVES - 1) / SHRINK_WAVES, p.tiles, ord), dim3(SHRINK_WAVES * 64), 0, st, p);
+        return;
+    }
+    const int groups = (p.n_pairs + 3) / 4;
+    const size_t lds = (size_t)p.max_chunks * 1024;
+    if (p.M <= SPREAD_ROWS) {
         hipLaunchKernelGGL((adapters_shrink_kernel<T, true>), dim3(p.tiles, p.splits, ord), dim3(SHRINK_WAVES * 64), 0, st, p);
-        hipLaunchKernelGGL((adapters_expand_kernel<T, 1, true>), dim3(p.tiles, (p.n_pairs + 3) / 4, ord), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((adapters_expand_kernel<T, 1, true>), dim3(p.tiles * groups, 1, ord), dim3(256), lds, st, p);
     } else {
         hipLaunchKernelGGL((adapters_shrink_kernel<T, false>), dim3(p.tiles, p.splits, 1), dim3(SHRINK_WAVES * 64), 0, st, p);
-        hipLaunchKernelGGL((adapters_expand_kernel<T, 4, false>), dim3((p.tiles + 3) / 4, (p.n_pairs + 3) / 4, 1), dim3(256), 0, st, p);
+        // four tiles of rows share a read of B once that still leaves every compute unit two workgroups
+        if ((int64_t)(p.tiles / 4) * groups >= 512)
+            hipLaunchKernelGGL((adapters_expand_kernel<T, 4, false>), dim3((p.tiles + 3) / 4 * groups), dim3(256), 4 * lds, st, p);
+        else
+            hipLaunchKernelGGL((adapters_expand_kernel<T, 1, false>), dim3(p.tiles * groups), dim3(256), lds, st, p);
     }
 }
 
@@ -337,19 +446,21 @@ extern "C" size_t sptmm_adapters_workspace_bytes(const sptmm_adapters *a, int M)
 extern "C" int sptmm_adapters_apply(const sptmm_adapters *a, const uint16_t *X, const int32_t *row_slot, int M, const float *base, float *Y, void *workspace,
                                     size_t workspace_bytes, void *stream)
 {
-    if (!a || !X || !row_slot || !Y || !workspace) return fail(SPTMM_ERR_INVALID, "null pointer");
+    if (!a || !X || !row_slot || !Y) return fail(SPTMM_ERR_INVALID, "null pointer");
     if (M < 1) return fail(SPTMM_ERR_INVALID, "M must be at least 1");
     if (M > (1 << 24)) return fail(SPTMM_ERR_INVALID, "M must be at most 2^24");
     if (((uintptr_t)X | (uintptr_t)base | (uintptr_t)Y | (uintptr_t)workspace) & 15) return fail(SPTMM_ERR_INVALID, "X, base, Y and the workspace must be aligned to 16 bytes");
     if ((uintptr_t)row_slot & 3) return fail(SPTMM_ERR_INVALID, "row_slot must be aligned to 4 bytes");
-    if (workspace_bytes < need(a, M)) return fail(SPTMM_ERR_INVALID, "the workspace has %zu bytes, %zu are needed", workspace_bytes, need(a, M));
+    const size_t want = need(a, M);
+    if (want && (!workspace || workspace_bytes < want))
+        return fail(SPTMM_ERR_INVALID, "the workspace has %zu bytes, %zu are needed", workspace ? workspace_bytes : (size_t)0, want);
     if (int rc = check_device(a)) return rc;
     AdapterArgs p{};
     p.X = X, p.A = a->A, p.B = a->B, p.row_slot = row_slot, p.chunks = a->chunks, p.scale = a->scale, p.base = base, p.h = (float *)workspace, p.Y = Y;
     p.M = M, p.K = a->K, p.N = a->N, p.slots = a->slots, p.k_steps = a->k_steps, p.n_pairs = a->n_pairs, p.max_chunks = a->max_chunks;
     p.tiles = (M + 15) / 16, p.splits = splits_of(a, M);
     const int ord = ordinals(M);
-    a->type == SPTMM_X_F16 ? launch_apply<SPTMM_X_F16>(p, ord, (hipStream_t)stream) : launch_apply<SPTMM_X_BF16>(p, ord, (hipStream_t)stream);
+    a->type == SPTMM_X_F16 ? launch_apply<SPTMM_X_F16>(p, fused(a, M), ord, (hipStream_t)stream) : launch_apply<SPTMM_X_BF16>(p, fused(a, M), ord, (hipStream_t)stream);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? SPTMM_OK : hip_fail(e, "adapters kernels launch");
 }

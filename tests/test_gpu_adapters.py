@@ -83,6 +83,17 @@ def test_shapes_and_ranks(K, N, t):
     s.free()
 
 
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("K,N,rank", [(2560, 3840, 16), (2576, 272, 9), (1024, 528, 75)])
+def test_a_few_rows(K, N, rank, t):
+    s = Set(10, K, N, t, [rank, 1, rank, 3, rank])
+    for M in (1, 2, 7, 16):
+        s.check(M, (np.arange(M) * 3 + 2) % 6 - 1)
+        s.check(M + 50, np.full(M, 2), "in place")
+    assert s.a.workspace_bytes(1) == 0  # small weights: both products in one launch
+    s.free()
+
+
 @pytest.mark.parametrize("rank,max_rank", [(1, 256), (64, 64), (65, 128), (200, 256), (256, 256)])
 def test_large_ranks(rank, max_rank):
     s = Set(3, 320, 96, "bf16", [rank, 5], max_rank)
@@ -178,16 +189,16 @@ def test_a_captured_call_follows_its_buffers():
 
 
 def test_refusals():
-    s = Set(9, 64, 32, "f16", [4, 4], 8)
+    s = Set(9, 6912, 32, "f16", [4, 4], 64)
     n = s.a.workspace_bytes(3)
     assert n > 0 and s.a.workspace_bytes(0) == 0 and s.a.workspace_bytes(-3) == 0
-    X, S, Y, ws = sp.DeviceBuffer(2 * 3 * 64 + 16), sp.DeviceBuffer(16), sp.DeviceBuffer(4 * 3 * 32 + 16), sp.DeviceBuffer(n + 16)
+    X, S, Y, ws = sp.DeviceBuffer(2 * 3 * 6912 + 16), sp.DeviceBuffer(16), sp.DeviceBuffer(4 * 3 * 32 + 16), sp.DeviceBuffer(n + 16)
     off = X.ptr.value + 2
     for a in ((None, S, 3, None, Y, ws, n), (X, None, 3, None, Y, ws, n), (X, S, 3, None, None, ws, n), (X, S, 3, None, Y, None, n), (X, S, 0, None, Y, ws, n), (X, S, -1, None, Y, ws, n),
               (X, S, 3, None, Y, ws, n - 1), (X, S, (1 << 24) + 1, None, Y, ws, n), (off, S, 3, None, Y, ws, n), (X, S.ptr.value + 2, 3, None, Y, ws, n), (X, S, 3, Y.ptr.value + 4, Y, ws, n)):
         with pytest.raises(sp.SptmmError):
             s.a.apply(*a)
-    for a in ((-1, X, Y, 4, 1.0), (2, X, Y, 4, 1.0), (0, X, Y, 9, 1.0), (0, X, Y, -1, 1.0), (0, None, Y, 4, 1.0), (0, X, None, 4, 1.0), (0, X, Y, 4, float("nan")), (0, X, Y, 4, float("inf"))):
+    for a in ((-1, X, Y, 4, 1.0), (2, X, Y, 4, 1.0), (0, X, Y, 65, 1.0), (0, X, Y, -1, 1.0), (0, None, Y, 4, 1.0), (0, X, None, 4, 1.0), (0, X, Y, 4, float("nan")), (0, X, Y, 4, float("inf"))):
         with pytest.raises(sp.SptmmError):
             s.a.set(*a)
     s.check(1, [0, 1, 0])
