@@ -12,10 +12,21 @@
 // and never by a product with zero: an infinity in one adapter's weights reaches its own rows only.
 //
 // Both weights sit in the order in which a wavefront reads them, 1 KiB per load instruction (adapters_pack_kernel).
+#include <atomic>
 #include <cmath>
 
 #include "internal.hpp"
 #include "lanes.hpp"
+
+namespace sptmm {
+// What the kernels know of a slot.  Its weights hold a value that is not finite where `bad` is the number of the call that set it
+// (found while packing, by many threads at once: they all write the same number, and none has to clear it first).
+struct SlotInfo {
+    int rank;  // 0: empty
+    float scale;
+    int set, bad;
+};
+}  // namespace sptmm
 
 struct sptmm_adapters {
     int K, N, type, slots, max_rank;
@@ -24,8 +35,8 @@ struct sptmm_adapters {
     int max_chunks;  // chunks of 16 ranks a slot has room for
     int device, compute_units;
     uint16_t *A, *B;  // [slot]: [chunk][k_step][64 lanes][8] and [n_pair][chunk][64 lanes][8], packed by the chunks in use
-    int *chunks;      // [slot] chunks of 16 ranks in use; 0: empty
-    float *scale;     // [slot]
+    sptmm::SlotInfo *info;
+    std::atomic<int> sets{0};  // calls of sptmm_adapters_set so far
 };
 
 namespace sptmm {
@@ -52,31 +63,35 @@ template <int T> __device__ __forceinline__ float widen(u16 b)
 
 struct AdapterArgs {
     const u16 *X, *A, *B;
-    const int *row_slot, *chunks;
-    const float *scale, *base;
+    const int *row_slot;
+    const SlotInfo *info;
+    const float *base;
     float *h, *Y;
-    int M, K, N, slots, k_steps, n_pairs, max_chunks, tiles, splits;
+    int M, K, N, slots, k_steps, n_pairs, max_chunks, tiles, splits, places;
 };
 
 // ------------------------------------------------------------------------------------------------ weights into place
 // One thread per stored value.  A lane of the first product's operand holds rank lane % 16, k = 8 * (lane / 16) + e of a step
 // of 32; of the second's, column lane % 16 (e < 4) or 16 + lane % 16 (e >= 4) of a pair, rank 4 * (lane / 16) + e % 4 of a chunk.
-__global__ void __launch_bounds__(256) adapters_pack_kernel(const u16 *A, const u16 *B, u16 *pA, u16 *pB, int *chunk_of, float *scale_of, int slot, int rank, float scale, int K,
-                                                            int N, int k_steps, int n_pairs, int chunks)
+__global__ void __launch_bounds__(256) adapters_pack_kernel(const u16 *A, const u16 *B, u16 *pA, u16 *pB, SlotInfo *info, int set, int rank, float scale, int K,
+                                                            int N, int k_steps, int n_pairs, int chunks, unsigned exponent)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i == 0) chunk_of[slot] = chunks, scale_of[slot] = scale;
+    if (i == 0) info->rank = rank, info->scale = scale, info->set = set;
     const int64_t na = (int64_t)chunks * k_steps * 512, nb = (int64_t)n_pairs * chunks * 512;
     const int e = (int)(i & 7), lane = (int)(i >> 3) & 63;
     if (i < na) {
         const int step = (int)((i >> 9) % k_steps), c = (int)((i >> 9) / k_steps);
         const int r = 16 * c + (lane & 15), k = 32 * step + 8 * (lane >> 4) + e;
-        pA[i] = r < rank && k < K ? A[(int64_t)r * K + k] : (u16)0;
+        const u16 x = r < rank && k < K ? A[(int64_t)r * K + k] : (u16)0;
+        pA[i] = x;
     }
     if (i < nb) {
         const int c = (int)((i >> 9) % chunks), pair = (int)((i >> 9) / chunks);
         const int n = 32 * pair + 16 * (e >> 2) + (lane & 15), r = 16 * c + 4 * (lane >> 4) + (e & 3);
-        pB[i] = r < rank && n < N ? B[(int64_t)n * rank + r] : (u16)0;
+        const u16 x = r < rank && n < N ? B[(int64_t)n * rank + r] : (u16)0;
+        pB[i] = x;
+        if ((x & exponent) == exponent) info->bad = set;
     }
 }
 
@@ -87,6 +102,8 @@ __device__ __forceinline__ int next_slot(int slot, unsigned long long &left)
     left &= ~__ballot(slot == s);
     return s;
 }
+
+__device__ __forceinline__ int chunks_of(int rank) { return (rank + 15) >> 4; }
 
 // slot of the row that this lane holds (row tile * 16 + lane % 16), -1 where it has none
 __device__ __forceinline__ int slot_of(const AdapterArgs &p, int m)
@@ -124,7 +141,7 @@ template <int T, int NC> __device__ __forceinline__ void walk_k(const AdapterArg
 
 // chunks c0 .. c0 + nc - 1 of slot s, summed over a range of K by the workgroup's eight wavefronts: afterwards wavefront w < nc
 // holds chunk c0 + w of all 16 rows.  The wavefronts' shares are added through the LDS in wavefront order.
-template <int T> __device__ __forceinline__ f32x4 shrink(const AdapterArgs &p, f32x4 (&sums)[SHRINK_WAVES][CHUNKS_AT_ONCE][64], int s, int c0, int nc, const u16 *x_row, int step0, int step1)
+template <int T> __device__ __forceinline__ f32x4 shrink(const AdapterArgs &p, f32x4 (&sums)[SHRINK_WAVES][CHUNKS_AT_ONCE][64], int s, int rank, int c0, int nc, const u16 *x_row, int step0, int step1)
 {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x4 acc[CHUNKS_AT_ONCE];
@@ -146,31 +163,33 @@ template <int T> __device__ __forceinline__ f32x4 shrink(const AdapterArgs &p, f
         t = sums[0][wave][lane];
 #pragma unroll
         for (int w = 1; w < SHRINK_WAVES; ++w) t += sums[w][wave][lane];
+        // ranks that only fill up the chunk: zeros whatever X holds (its infinities times their zeros are none)
+        const int r = 16 * (c0 + wave) + 4 * (lane >> 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = r + e < rank ? t[e] : 0.f;
     }
     return t;
 }
 
-// Workgroup (tile of 16 rows, split of K, ordinal of a distinct slot in the tile).  ONE: it serves one slot of its tile (few rows:
-// slots spread over workgroups); else it walks them all.
-template <int T, bool ONE> __global__ void __launch_bounds__(SHRINK_WAVES * 64) adapters_shrink_kernel(const AdapterArgs p)
+// Workgroup (tile of 16 rows, split of K, group of four chunks and place among the tile's distinct slots): it serves every
+// `places`-th distinct slot of the tile.
+template <int T> __global__ void __launch_bounds__(SHRINK_WAVES * 64) adapters_shrink_kernel(const AdapterArgs p)
 {
     __shared__ __attribute__((aligned(16))) f32x4 sums[SHRINK_WAVES][CHUNKS_AT_ONCE][64];
     const int tile = blockIdx.x, split = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c0 = (int)(blockIdx.z / p.places) * CHUNKS_AT_ONCE, place = (int)(blockIdx.z % p.places);
     const int m = tile * 16 + (lane & 15), slot = slot_of(p, m);
     unsigned long long left = __ballot(slot >= 0) & 0xffff;
-    if (ONE)
-        for (int o = blockIdx.z; o > 0 && left; --o) next_slot(slot, left);
     const int per = (p.k_steps + p.splits - 1) / p.splits, step0 = split * per, step1 = min(p.k_steps, step0 + per);
     const u16 *x_row = p.X + (int64_t)min(m, p.M - 1) * p.K + 8 * (lane >> 4);
-    while (left) {
-        const int s = next_slot(slot, left), chunks = p.chunks[s];
-        for (int c0 = 0; c0 < chunks; c0 += CHUNKS_AT_ONCE) {
-            const int nc = min(CHUNKS_AT_ONCE, chunks - c0);
-            const f32x4 t = shrink<T>(p, sums, s, c0, nc, x_row, step0, step1);
-            if (wave < nc && slot == s) reinterpret_cast<f32x4 *>(p.h)[(((int64_t)split * p.tiles + tile) * p.max_chunks + c0 + wave) * 64 + lane] = t;
-            __syncthreads();
-        }
-        if (ONE) break;
+    for (int o = 0; left; ++o) {
+        const int s = next_slot(slot, left);
+        if (o % p.places != place) continue;
+        const int rank = p.info[s].rank, nc = min(CHUNKS_AT_ONCE, chunks_of(rank) - c0);
+        if (nc <= 0) continue;
+        const f32x4 t = shrink<T>(p, sums, s, rank, c0, nc, x_row, step0, step1);
+        if (wave < nc && slot == s) reinterpret_cast<f32x4 *>(p.h)[(((int64_t)split * p.tiles + tile) * p.max_chunks + c0 + wave) * 64 + lane] = t;
+        __syncthreads();
     }
 }
 
@@ -187,100 +206,193 @@ template <int T> __device__ __forceinline__ void add_chunk(u16x8 b, f32x4 h, boo
 #pragma unroll
     for (int e = 0; e < 4; ++e) y0[e] = mine ? n0[e] : y0[e], y1[e] = mine ? n1[e] : y1[e];
 }
+// The same on the 16-bit matrix instruction, an eighth (fp16) or a quarter (bf16) of its time: where many rows make the second product
+// long enough to stand beside its bytes.  A 32-bit h is the sum of parts of 16 bits, which share an instruction's 32 places along
+// the contraction with B's values given twice: three parts of bf16 are h exactly; of fp16, whose range is short, a row's h
+// is first brought below 2^15 by a power of two, and two parts hold 22 bits of it.  An h that is not finite is its first part; a
+// B that is not finite would meet the other parts' signs and zeros, and goes the 32-bit way.
+template <int T> struct Parts {
+    float top = 0.f, scale = 1.f, back = 1.f;  // fp16: largest |h| of this lane's row, the power of two, and the way back
+    u16x8 first;
+    u16x8 third;
+
+    __device__ __forceinline__ void add(f32x4 h)
+    {
+        if constexpr (T == SPTMM_X_F16)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fabsf(h[e]) < INFINITY ? fmaxf(top, fabsf(h[e])) : top;
+    }
+    __device__ __forceinline__ void settle()
+    {
+        if constexpr (T == SPTMM_X_F16) {  // (a row's four lanes)
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const int e = max((int)(__builtin_bit_cast(unsigned, top) >> 23), 27) - 127 - 14;  // top < 2^(e + 15)
+            scale = __builtin_bit_cast(float, (unsigned)(127 - e) << 23);
+            back = __builtin_bit_cast(float, (unsigned)(127 + e) << 23);
+        }
+    }
+    __device__ __forceinline__ void split(f32x4 h)
+    {
+        third = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = h[e];
+            if constexpr (T == SPTMM_X_F16) {
+                const float y = x * scale;
+                const _Float16 hi = (_Float16)y;
+                const _Float16 lo = fabsf(y) < INFINITY ? (_Float16)(y - (float)hi) : (_Float16)0.f;
+                first[e] = __builtin_bit_cast(u16, hi), first[4 + e] = __builtin_bit_cast(u16, lo);
+            } else {
+                const bool finite = fabsf(x) < INFINITY;
+                const unsigned hi = __builtin_bit_cast(unsigned, x) & 0xffff0000u;
+                const float r = finite ? x - __builtin_bit_cast(float, hi) : 0.f;
+                const unsigned mid = __builtin_bit_cast(unsigned, r) & 0xffff0000u;
+                const float rest = r - __builtin_bit_cast(float, mid);
+                first[e] = (u16)(hi >> 16), first[4 + e] = (u16)(mid >> 16), third[e] = (u16)(__builtin_bit_cast(unsigned, rest) >> 16);
+            }
+        }
+    }
+    __device__ __forceinline__ void add_chunk(u16x8 b, bool mine, f32x4 &y0, f32x4 &y1) const
+    {
+        const u16x8 b0 = __builtin_shufflevector(b, b, 0, 1, 2, 3, 0, 1, 2, 3), b1 = __builtin_shufflevector(b, b, 4, 5, 6, 7, 4, 5, 6, 7);
+        f32x4 n0 = mfma16<T>(b0, first, y0), n1 = mfma16<T>(b1, first, y1);
+        if constexpr (T != SPTMM_X_F16) n0 = mfma16<T>(b0, third, n0), n1 = mfma16<T>(b1, third, n1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y0[e] = mine ? n0[e] : y0[e], y1[e] = mine ? n1[e] : y1[e];
+    }
+};
 // the operand of column pair `pair`, chunk c of slot s (`chunks` chunks in use)
 __device__ __forceinline__ u16x8 load_b(const AdapterArgs &p, int s, int pair, int chunks, int c)
 {
     return *reinterpret_cast<const u16x8 *>(p.B + ((int64_t)s * p.n_pairs * p.max_chunks + (int64_t)pair * chunks + c) * 512 + (threadIdx.x & 63) * 8);
 }
 
-// A workgroup takes 16 * RT rows and its four wavefronts 32 columns each.  Every row's h (its own slot's) is first brought into the
-// LDS, scaled and with the splits' partial sums added in their order; then the distinct slots are walked.
-// ONE (RT = 1): only the rows of one distinct slot of the tile (and, the first of them, the rows without a slot).
-template <int T, int RT, bool ONE> __global__ void __launch_bounds__(256) adapters_expand_kernel(const AdapterArgs p)
+// A wavefront takes one tile of 16 rows and CP pairs of 16 columns.  The four wavefronts of a workgroup take neighbouring columns
+// of one tile or (ROWS) the same columns of four tiles: few rows need many workgroups, and many rows are bound by base and Y, of
+// which a wavefront then moves 512 bytes of every row.  The rows' h (each row its own slot's) is first brought into the LDS,
+// scaled and with the splits' partial sums added in their order; then the distinct slots are walked.
+// Without ROWS the distinct slots of a tile are shared by `places` workgroups, which write the rows of their own.
+template <int T, int CP, bool ROWS> __global__ void __launch_bounds__(256) adapters_expand_kernel(const AdapterArgs p)
 {
-    extern __shared__ __attribute__((aligned(16))) f32x4 h_lds[];  // [RT][max_chunks][64]
+    extern __shared__ __attribute__((aligned(16))) f32x4 h_lds[];  // [ROWS ? 4 : 1][max_chunks][64]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int groups = (p.n_pairs + 3) / 4, tile0 = (int)(blockIdx.x / groups) * RT, pair = (int)(blockIdx.x % groups) * 4 + wave;
-    int slot[RT], chunks_of[RT];
-    bool write[RT];
-    unsigned long long left[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int m = (tile0 + t) * 16 + (lane & 15);
-        slot[t] = slot_of(p, m);
-        left[t] = __ballot(slot[t] >= 0) & 0xffff;
-        write[t] = m < p.M;
+    const int per = (ROWS ? 1 : 4) * CP, groups = (p.n_pairs + per - 1) / per;
+    const int tile = (int)(blockIdx.x / groups) * (ROWS ? 4 : 1) + (ROWS ? wave : 0);
+    const int pair = (int)(blockIdx.x % groups) * per + (ROWS ? 0 : wave * CP);
+    const int m = tile * 16 + (lane & 15), slot = slot_of(p, m);
+    unsigned long long left = __ballot(slot >= 0) & 0xffff;
+    bool write = m < p.M;
+    if (!ROWS && p.places > 1) {  // the slots of this workgroup's place, and for the first place the rows without a slot
+        unsigned long long rest = left;
+        left = 0;
+        for (int o = 0; rest; ++o) {
+            const unsigned long long before = rest;
+            next_slot(slot, rest);
+            if (o % p.places == (int)blockIdx.z) left |= before & ~rest;
+        }
+        if (!left && blockIdx.z) return;
+        write = write && (slot >= 0 ? (left >> (lane & 15) & 1) != 0 : blockIdx.z == 0);
     }
-    if (ONE) {
-        for (int o = blockIdx.z; o > 0 && left[0]; --o) next_slot(slot[0], left[0]);
-        if (!left[0] && blockIdx.z) return;
-        const int mine = left[0] ? __builtin_amdgcn_readlane(slot[0], __builtin_ctzll(left[0])) : -2;
-        write[0] = write[0] && (slot[0] == mine || (blockIdx.z == 0 && slot[0] < 0));
-        left[0] &= __ballot(slot[0] == mine);
-    }
-    const int n0 = pair * 32 + 4 * (lane >> 4);
-    const bool first = pair < p.n_pairs, second = pair * 32 + 16 < p.N;  // (an odd number of 16-column groups: the last pair has one)
-    f32x4 acc[RT][2];
+    const int64_t at = (int64_t)m * p.N + pair * 32 + 4 * (lane >> 4);
+    const int cols = (p.N - pair * 32) / 16;  // groups of 16 columns from here on
+    f32x4 acc[CP][2];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int64_t at = (int64_t)((tile0 + t) * 16 + (lane & 15)) * p.N + n0;
+    for (int c = 0; c < CP; ++c)
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            acc[t][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (p.base && write[t] && (g ? second : first)) acc[t][g] = *reinterpret_cast<const f32x4 *>(p.base + at + 16 * g);
+            acc[c][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (p.base && write && 2 * c + g < cols) acc[c][g] = *reinterpret_cast<const f32x4 *>(p.base + at + 32 * c + 16 * g);
         }
-    }
+    // the walk's place: DEEP chunks from c on of slot s (s < 0: the walk is over); its first B is on its way while h is brought in
+    constexpr int DEEP = ROWS ? 1 : 4;
+    struct Place {
+        int s, chunks, c;
+    };
+    auto after = [&](Place at) {
+        if ((at.c += DEEP) < at.chunks) return at;
+        at.c = 0;
+        do {
+            at.s = left ? next_slot(slot, left) : -1;
+            at.chunks = at.s >= 0 ? chunks_of(p.info[at.s].rank) : 0;
+        } while (at.s >= 0 && at.chunks == 0);
+        return at;
+    };
+    auto load = [&](const Place &at, u16x8(&b)[DEEP][CP]) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        chunks_of[t] = slot[t] >= 0 && write[t] ? p.chunks[slot[t]] : 0;
-        const float scale = chunks_of[t] ? p.scale[slot[t]] : 0.f;
-        for (int c = wave; c < p.max_chunks; c += 4) {
-            if (!__ballot(c < chunks_of[t])) break;
-            if (c < chunks_of[t]) {
-                const f32x4 *hp = reinterpret_cast<const f32x4 *>(p.h) + ((int64_t)(tile0 + t) * p.max_chunks + c) * 64 + lane;
-                const int64_t next = (int64_t)p.tiles * p.max_chunks * 64;
-                f32x4 h = hp[0];
-                int k = 1;
-                for (; k + 4 <= p.splits; k += 4) {
-                    const f32x4 a = hp[k * next], b = hp[(k + 1) * next], c4 = hp[(k + 2) * next], d = hp[(k + 3) * next];
-                    h += a, h += b, h += c4, h += d;
-                }
-                for (; k < p.splits; ++k) h += hp[k * next];
-                h_lds[(t * p.max_chunks + c) * 64 + lane] = h * scale;
+        for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+            for (int i = 0; i < CP; ++i)
+                if (at.s >= 0 && 2 * i < cols) b[d][i] = load_b(p, at.s, pair + i, at.chunks, min(at.c + d, at.chunks - 1));
+    };
+    Place now = after(Place{-1, 0, 0});
+    u16x8 b[DEEP][CP];
+    load(now, b);
+
+    const SlotInfo mine = slot >= 0 && write ? p.info[slot] : SlotInfo{0, 0.f, 0, 0};
+    const int my_chunks = chunks_of(mine.rank);
+    const unsigned long long wide = __ballot(mine.rank && mine.bad == mine.set);  // rows whose B takes the 32-bit instruction
+    Parts<T> big;
+    f32x4 *const h_tile = h_lds + (ROWS ? wave * p.max_chunks * 64 : 0);
+    for (int c = ROWS ? 0 : wave; c < p.max_chunks; c += ROWS ? 1 : 4) {
+        if (!__ballot(c < my_chunks)) break;
+        if (c < my_chunks) {
+            const f32x4 *hp = reinterpret_cast<const f32x4 *>(p.h) + ((int64_t)tile * p.max_chunks + c) * 64 + lane;
+            const int64_t next = (int64_t)p.tiles * p.max_chunks * 64;
+            f32x4 h = hp[0];
+            int k = 1;
+            for (; k + 4 <= p.splits; k += 4) {
+                const f32x4 a = hp[k * next], b = hp[(k + 1) * next], c4 = hp[(k + 2) * next], d = hp[(k + 3) * next];
+                h += a, h += b, h += c4, h += d;
             }
+            for (; k < p.splits; ++k) h += hp[k * next];
+            h *= mine.scale;
+            h_tile[c * 64 + lane] = h;
+            if constexpr (ROWS) big.add(h);
         }
     }
     __syncthreads();
-    if (!first) return;
+    if (cols <= 0) return;
+    if constexpr (ROWS) big.settle();
+    // (fp16 parts are scaled: their sums stand apart until the end)
+    constexpr bool APART = ROWS && T == SPTMM_X_F16;
+    f32x4 sum[CP][2];
+    if constexpr (APART)
 #pragma unroll
-    for (int t0 = 0; t0 < RT; ++t0) {
-        while (left[t0]) {  // distinct slots of all the rows: those of a later tile are served with the first tile that has them
-            const int s = next_slot(slot[t0], left[t0]), chunks = p.chunks[s];
-            bool has[RT];
+        for (int c = 0; c < CP; ++c) sum[c][0] = sum[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    while (now.s >= 0) {
+        const Place then = after(now);
+        u16x8 next[DEEP][CP];
+        load(then, next);
+        const bool serves = slot == now.s, parts = ROWS && !(wide & __ballot(serves));
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                const unsigned long long b = __ballot(slot[t] == s) & 0xffff;
-                has[t] = t >= t0 && b;
-                if (t > t0) left[t] &= ~b;
-            }
-            u16x8 b = load_b(p, s, pair, chunks, 0);
-            for (int c = 0; c < chunks; ++c) {
-                const u16x8 now = b;
-                if (c + 1 < chunks) b = load_b(p, s, pair, chunks, c + 1);
+        for (int d = 0; d < DEEP; ++d) {
+            if (now.c + d >= now.chunks) break;
+            const f32x4 h = h_tile[(now.c + d) * 64 + lane];
+            if (parts) big.split(h);
 #pragma unroll
-                for (int t = 0; t < RT; ++t)
-                    if (has[t]) add_chunk<T>(now, h_lds[(t * p.max_chunks + c) * 64 + lane], slot[t] == s, acc[t][0], acc[t][1]);
-            }
+            for (int i = 0; i < CP; ++i)
+                if (2 * i < cols) {
+                    if (!parts) add_chunk<T>(b[d][i], h, serves, acc[i][0], acc[i][1]);
+                    else if constexpr (APART) big.add_chunk(b[d][i], serves, sum[i][0], sum[i][1]);
+                    else big.add_chunk(b[d][i], serves, acc[i][0], acc[i][1]);
+                }
         }
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+            for (int i = 0; i < CP; ++i) b[d][i] = next[d][i];
+        now = then;
     }
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int64_t at = (int64_t)((tile0 + t) * 16 + (lane & 15)) * p.N + n0;
-        if (write[t]) {
-            *reinterpret_cast<f32x4 *>(p.Y + at) = acc[t][0];
-            if (second) *reinterpret_cast<f32x4 *>(p.Y + at + 16) = acc[t][1];
+    for (int c = 0; c < CP; ++c)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            if constexpr (APART)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[c][g][e] = fmaf(sum[c][g][e], big.back, acc[c][g][e]);
+            if (write && 2 * c + g < cols) *reinterpret_cast<f32x4 *>(p.Y + at + 32 * c + 16 * g) = acc[c][g];
         }
-    }
 }
 
 // ------------------------------------------------------------------------------------------------ both products in one launch
@@ -294,7 +406,7 @@ template <int T> __global__ void __launch_bounds__(SHRINK_WAVES * 64) adapters_f
     unsigned long long left = __ballot(slot >= 0) & 0xffff;
     for (int o = blockIdx.z; o > 0 && left; --o) next_slot(slot, left);
     if (!left && blockIdx.z) return;
-    const int s = left ? __builtin_amdgcn_readlane(slot, __builtin_ctzll(left)) : -2, chunks = left ? p.chunks[s] : 0;
+    const int s = left ? __builtin_amdgcn_readlane(slot, __builtin_ctzll(left)) : -2, rank = left ? p.info[s].rank : 0, chunks = chunks_of(rank);
     const bool write = m < p.M && (slot == s || (blockIdx.z == 0 && slot < 0));
     const int n0 = pair * 32 + 4 * (lane >> 4);
     const bool first = pair < p.n_pairs, second = pair * 32 + 16 < p.N;
@@ -302,7 +414,7 @@ template <int T> __global__ void __launch_bounds__(SHRINK_WAVES * 64) adapters_f
     f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     if (p.base && write && first) acc[0] = *reinterpret_cast<const f32x4 *>(p.base + at);
     if (p.base && write && second) acc[1] = *reinterpret_cast<const f32x4 *>(p.base + at + 16);
-    const float scale = chunks ? p.scale[s] : 0.f;
+    const float scale = chunks ? p.info[s].scale : 0.f;
     const u16 *x_row = p.X + (int64_t)min(m, p.M - 1) * p.K + 8 * (lane >> 4);
     for (int c0 = 0; c0 < chunks; c0 += CHUNKS_AT_ONCE) {
         const int nc = min(CHUNKS_AT_ONCE, chunks - c0);
@@ -310,7 +422,7 @@ template <int T> __global__ void __launch_bounds__(SHRINK_WAVES * 64) adapters_f
         if (first)
 #pragma unroll
             for (int c = 0; c < CHUNKS_AT_ONCE; ++c) b[c] = load_b(p, s, pair, chunks, min(c0 + c, chunks - 1));
-        const f32x4 t = shrink<T>(p, sums, s, c0, nc, x_row, 0, p.k_steps);
+        const f32x4 t = shrink<T>(p, sums, s, rank, c0, nc, x_row, 0, p.k_steps);
         if (wave < nc) h_lds[wave][lane] = t * scale;
         __syncthreads();
         if (first)
@@ -324,19 +436,19 @@ template <int T> __global__ void __launch_bounds__(SHRINK_WAVES * 64) adapters_f
 
 int hip_fail(hipError_t e, const char *what) { return fail(SPTMM_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e); }
 
-// Up to this many rows the distinct slots of a tile go to workgroups of their own (decode: every row may have another one, and a
-// workgroup that walks sixteen waits for sixteen chains of loads); beyond it, prompts, a tile rarely has more than two.
-constexpr int SPREAD_ROWS = 128;
 // Up to this much of A (KiB of the largest slot), and one tile of rows, both products run in one launch.
 constexpr int FUSED_A_KIB = 160;
 
-int ordinals(int M) { return M <= SPREAD_ROWS ? (M < 16 ? M : 16) : 1; }
 bool fused(const sptmm_adapters *a, int M) { return M <= 16 && a->max_chunks * a->k_steps <= FUSED_A_KIB; }
+
+// Workgroups that share the distinct slots of a tile.  Decode: every row may have another slot, and a workgroup that walks sixteen
+// waits for sixteen chains of loads; prompts: a tile rarely has more than two, and workgroups that find none cost their launch.
+int places_of(int M) { return M < 16 ? M : M <= 128 ? 16 : M <= 1024 ? 4 : 2; }
 
 // splits of K over workgroups: enough of them to fill the chip, each wavefront with two steps of 32 at least
 int splits_of(const sptmm_adapters *a, int M)
 {
-    const int tiles = (M + 15) / 16, groups = tiles * ordinals(M);
+    const int tiles = (M + 15) / 16, groups = tiles * (M <= 128 ? places_of(M) : 1);
     const int want = (a->compute_units + groups - 1) / groups, most = (a->k_steps + 2 * SHRINK_WAVES - 1) / (2 * SHRINK_WAVES);
     return want < 1 ? 1 : want < most ? want : most;
 }
@@ -355,25 +467,19 @@ int check_device(const sptmm_adapters *a)
     return SPTMM_OK;
 }
 
-template <int T> void launch_apply(const AdapterArgs &p, bool one_launch, int ord, hipStream_t st)
+template <int T> void launch_apply(const AdapterArgs &p, bool one_launch, hipStream_t st)
 {
     if (one_launch) {
-        hipLaunchKernelGGL((adapters_fused_kernel<T>), dim3((p.n_pairs + SHRINK_WAVES - 1) / SHRINK_WAVES, p.tiles, ord), dim3(SHRINK_WAVES * 64), 0, st, p);
+        hipLaunchKernelGGL((adapters_fused_kernel<T>), dim3((p.n_pairs + SHRINK_WAVES - 1) / SHRINK_WAVES, p.tiles, p.places), dim3(SHRINK_WAVES * 64), 0, st, p);
         return;
     }
-    const int groups = (p.n_pairs + 3) / 4;
+    const int groups = (p.n_pairs + 3) / 4, z = p.places * ((p.max_chunks + CHUNKS_AT_ONCE - 1) / CHUNKS_AT_ONCE);
     const size_t lds = (size_t)p.max_chunks * 1024;
-    if (p.M <= SPREAD_ROWS) {
-        hipLaunchKernelGGL((adapters_shrink_kernel<T, true>), dim3(p.tiles, p.splits, ord), dim3(SHRINK_WAVES * 64), 0, st, p);
-        hipLaunchKernelGGL((adapters_expand_kernel<T, 1, true>), dim3(p.tiles * groups, 1, ord), dim3(256), lds, st, p);
-    } else {
-        hipLaunchKernelGGL((adapters_shrink_kernel<T, false>), dim3(p.tiles, p.splits, 1), dim3(SHRINK_WAVES * 64), 0, st, p);
-        // four tiles of rows share a read of B once that still leaves every compute unit two workgroups
-        if ((int64_t)(p.tiles / 4) * groups >= 512)
-            hipLaunchKernelGGL((adapters_expand_kernel<T, 4, false>), dim3((p.tiles + 3) / 4 * groups), dim3(256), 4 * lds, st, p);
-        else
-            hipLaunchKernelGGL((adapters_expand_kernel<T, 1, false>), dim3(p.tiles * groups), dim3(256), lds, st, p);
-    }
+    hipLaunchKernelGGL((adapters_shrink_kernel<T>), dim3(p.tiles, p.splits, z), dim3(SHRINK_WAVES * 64), 0, st, p);
+    if ((int64_t)(p.tiles / 4) * groups < 512)  // (of the other kind there would be fewer than two workgroups per compute unit)
+        hipLaunchKernelGGL((adapters_expand_kernel<T, 1, false>), dim3(p.tiles * groups, 1, p.places), dim3(256), lds, st, p);
+    else
+        hipLaunchKernelGGL((adapters_expand_kernel<T, 4, true>), dim3((p.tiles + 3) / 4 * groups), dim3(256), 4 * lds, st, p);
 }
 
 }  // namespace
@@ -386,8 +492,7 @@ extern "C" void sptmm_adapters_free(sptmm_adapters *a)
     if (!a) return;
     if (a->A) (void)hipFree(a->A);
     if (a->B) (void)hipFree(a->B);
-    if (a->chunks) (void)hipFree(a->chunks);
-    if (a->scale) (void)hipFree(a->scale);
+    if (a->info) (void)hipFree(a->info);
     delete a;
 }
 
@@ -408,9 +513,8 @@ extern "C" int sptmm_adapters_create(int K, int N, int type, int slots, int max_
     if (e == hipSuccess) e = hipDeviceGetAttribute(&a->compute_units, hipDeviceAttributeMultiprocessorCount, a->device);
     if (e == hipSuccess) e = hipMalloc((void **)&a->A, per_a * slots);
     if (e == hipSuccess) e = hipMalloc((void **)&a->B, per_b * slots);
-    if (e == hipSuccess) e = hipMalloc((void **)&a->chunks, sizeof(int) * slots);
-    if (e == hipSuccess) e = hipMalloc((void **)&a->scale, sizeof(float) * slots);
-    if (e == hipSuccess) e = hipMemset(a->chunks, 0, sizeof(int) * slots);
+    if (e == hipSuccess) e = hipMalloc((void **)&a->info, sizeof(SlotInfo) * slots);
+    if (e == hipSuccess) e = hipMemset(a->info, 0, sizeof(SlotInfo) * slots);
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
         sptmm_adapters_free(a);
@@ -431,8 +535,8 @@ extern "C" int sptmm_adapters_set(sptmm_adapters *a, int slot, const uint16_t *A
     const int chunks = (rank + 15) / 16;
     const int64_t n = (int64_t)chunks * 512 * std::max(a->k_steps, a->n_pairs);
     u16 *pA = a->A + (size_t)slot * a->max_chunks * a->k_steps * 512, *pB = a->B + (size_t)slot * a->max_chunks * a->n_pairs * 512;
-    hipLaunchKernelGGL(adapters_pack_kernel, dim3((unsigned)std::max<int64_t>(1, (n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, A, B, pA, pB, a->chunks, a->scale, slot, rank,
-                       scale, a->K, a->N, a->k_steps, a->n_pairs, chunks);
+    hipLaunchKernelGGL(adapters_pack_kernel, dim3((unsigned)std::max<int64_t>(1, (n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, A, B, pA, pB, a->info + slot,
+                       (a->sets++ & 0x3fffffff) + 1, rank, scale, a->K, a->N, a->k_steps, a->n_pairs, chunks, a->type == SPTMM_X_F16 ? 0x7c00u : 0x7f80u);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? SPTMM_OK : hip_fail(e, "adapters_pack_kernel launch");
 }
@@ -456,11 +560,10 @@ extern "C" int sptmm_adapters_apply(const sptmm_adapters *a, const uint16_t *X, 
         return fail(SPTMM_ERR_INVALID, "the workspace has %zu bytes, %zu are needed", workspace ? workspace_bytes : (size_t)0, want);
     if (int rc = check_device(a)) return rc;
     AdapterArgs p{};
-    p.X = X, p.A = a->A, p.B = a->B, p.row_slot = row_slot, p.chunks = a->chunks, p.scale = a->scale, p.base = base, p.h = (float *)workspace, p.Y = Y;
+    p.X = X, p.A = a->A, p.B = a->B, p.row_slot = row_slot, p.info = a->info, p.base = base, p.h = (float *)workspace, p.Y = Y;
     p.M = M, p.K = a->K, p.N = a->N, p.slots = a->slots, p.k_steps = a->k_steps, p.n_pairs = a->n_pairs, p.max_chunks = a->max_chunks;
-    p.tiles = (M + 15) / 16, p.splits = splits_of(a, M);
-    const int ord = ordinals(M);
-    a->type == SPTMM_X_F16 ? launch_apply<SPTMM_X_F16>(p, fused(a, M), ord, (hipStream_t)stream) : launch_apply<SPTMM_X_BF16>(p, fused(a, M), ord, (hipStream_t)stream);
+    p.tiles = (M + 15) / 16, p.splits = splits_of(a, M), p.places = places_of(M);
+    a->type == SPTMM_X_F16 ? launch_apply<SPTMM_X_F16>(p, fused(a, M), (hipStream_t)stream) : launch_apply<SPTMM_X_BF16>(p, fused(a, M), (hipStream_t)stream);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? SPTMM_OK : hip_fail(e, "adapters kernels launch");
 }

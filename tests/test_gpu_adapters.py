@@ -61,7 +61,8 @@ class Set:
         with np.errstate(invalid="ignore"):
             want, bound = op.adapters(x64, slot, np.zeros((M, self.N)) if base == "none" else b32.astype(np.float64), self.A, self.B, self.scale)
         fine = np.isfinite(want)
-        assert (np.isnan(got) == np.isnan(want)).all()
+        bad = np.argwhere(np.isnan(got) != np.isnan(want))
+        assert not len(bad), (len(bad), bad[:3], got[tuple(bad[0])], want[tuple(bad[0])], slot[bad[0][0]])
         assert (got[~fine & ~np.isnan(want)] == want[~fine & ~np.isnan(want)]).all()
         off = np.abs(got - want)
         assert (off[fine] <= bound[fine]).all(), float((off[fine] / bound[fine]).max())
@@ -91,6 +92,26 @@ def test_a_few_rows(K, N, rank, t):
         s.check(M, (np.arange(M) * 3 + 2) % 6 - 1)
         s.check(M + 50, np.full(M, 2), "in place")
     assert s.a.workspace_bytes(1) == 0  # small weights: both products in one launch
+    s.free()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_many_rows(t):
+    """Enough rows and columns for the second product on the 16-bit matrix instruction, by parts of h."""
+    s = Set(11, 48, 2064, t, [1, 16, 40, 7, 64])
+    r = np.random.default_rng(1)
+    M = 2100
+    s.check(1, np.sort(r.integers(-1, 6, M)))
+    s.check(2, r.integers(-1, 6, M), "in place")
+
+    def spread(x):  # sums of very different size, and rows that are not finite
+        x[::3] *= 1e4 if t == "f16" else 1e20
+        x[1::3] *= 1e-4 if t == "f16" else 1e-20
+        x[2, 3], x[900, 0], x[1500, 7] = np.inf, np.nan, -np.inf
+        x[40] = 0.0
+    s.check(3, np.arange(M) // 40 % 6, edit=spread)
+    s.put(1, r, 16, edit=lambda A, B: B.__setitem__((70, 3), np.inf))
+    s.check(4, np.arange(M) // 9 % 6 - 1)
     s.free()
 
 
