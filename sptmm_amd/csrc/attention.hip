@@ -118,6 +118,55 @@ template <int LOG_TM> __device__ __forceinline__ bool find_tile(const AttnParams
     return true;
 }
 
+// The same in the order of the tiles' last keys, the furthest first, over all sequences: a tile's work is proportional to the keys it
+// sees, and workgroups that are dispatched late should be short.  Tile t of a sequence is placed at v = t + (keys before its
+// queries, in tiles); sequence b covers the places off .. off + tiles - 1.  With a sequence in every lane, the place of tile
+// `rank` is found by evaluating, at 64 places at a time, how many tiles lie at or behind the place.
+constexpr int BY_WORK = 32;  // sequences, at most (the evaluation walks them)
+template <int LOG_TM> __device__ __forceinline__ bool find_tile_by_work(const AttnParams &p, int rank, Tile *t)
+{
+    const int lane = threadIdx.x & 63, b = min(lane, p.batch - 1);
+    const int q0 = min(max(p.q_start[b], 0), p.total_q), q1 = min(max(p.q_start[b + 1], 0), p.total_q), nq = max(q1 - q0, 0);
+    const int k0 = p.kv_start ? p.kv_start[b] : q0;
+    int nk = p.kv_len ? p.kv_len[b] : nq;
+    if (k0 < 0 || k0 >= p.kv_rows) nk = 0;
+    const int first = nk > 0 ? k0 : 0;
+    nk = (int)min((int64_t)max(nk, 0), p.kv_rows - first);
+    const int tiles = lane < p.batch ? (int)(((int64_t)nq * p.group + (1 << LOG_TM) - 1) >> LOG_TM) : 0;
+    const int off = (int)(((int64_t)(nk - nq) * p.group) >> LOG_TM), behind = off + tiles;
+    int lo = 0x7fffffff, hi = -0x7fffffff;
+    for (int i = 0; i < p.batch; ++i)
+        if (__builtin_amdgcn_readlane(tiles, i) > 0) {
+            lo = min(lo, __builtin_amdgcn_readlane(off, i));
+            hi = max(hi, __builtin_amdgcn_readlane(behind, i));
+        }
+    if (lo >= hi) return false;
+    int64_t count;
+    int at;
+    for (int64_t stride = ((int64_t)hi - lo + 63) / 64;; stride = (stride + 63) / 64) {
+        const int64_t v = lo + lane * stride;
+        count = 0;
+        for (int i = 0; i < p.batch; ++i)
+            count += min(max((int64_t)__builtin_amdgcn_readlane(behind, i) - v, (int64_t)0), (int64_t)__builtin_amdgcn_readlane(tiles, i));
+        const int c = __popcll(__ballot(count > rank));
+        if (c == 0) return false;  // (there are no more than `rank` tiles)
+        at = c - 1;
+        if (stride == 1) break;
+        lo += (int)(at * stride);
+    }
+    const int place = lo + at, have = (int)__shfl((long long)count, at, 64);
+    unsigned long long who = __ballot(lane < p.batch && off <= place && place < behind);
+    for (int r = rank - (have - __popcll(who)); r > 0; --r) who &= who - 1;
+    const int seq = __builtin_amdgcn_readfirstlane(__builtin_ctzll(who));
+    t->q0 = __builtin_amdgcn_readlane(q0, seq);
+    t->nq = __builtin_amdgcn_readlane(nq, seq);
+    t->k0 = __builtin_amdgcn_readlane(first, seq);
+    t->nk = __builtin_amdgcn_readlane(nk, seq);
+    t->rows = t->nq * p.group;
+    t->row0 = (place - __builtin_amdgcn_readlane(off, seq)) << LOG_TM;
+    return true;
+}
+
 // ------------------------------------------------------------------------------------------------ tiles in the LDS
 // A tile is KT rows of DP values in row order; the 16-byte pieces of a row are permuted among themselves by a function of
 // the row so that the reads below meet different banks: K is read 16 bytes a lane, one piece of 32 rows at a time; V four
@@ -196,27 +245,36 @@ template <int T, int DP, int KT> struct Rows {
     {
         if (min(j0 + KT, end) - 1 <= lo) return false;
         const int lane = threadIdx.x & 63;
-        bool bad = false;
-        constexpr unsigned E = T == SPTMM_X_F16 ? 0x7c00u : 0x7f80u;
-        for (int i = lane; i < KT * DP / 8; i += 64) {
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(v + i * 16);
+        // the largest magnitude of all the values' bits, as integers: an exponent of ones is above every finite value's
+        typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+        u16x2 most = {0, 0};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bad = bad || (w[j] & E) == E || (w[j] & E << 16) == E << 16;
+        for (int i = 0; i < KT * DP / 512; ++i) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(v + (i * 64 + lane) * 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned x = w[j] & 0x7fff7fffu;
+                most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x));
+            }
         }
-        return __ballot(bad) != 0;
+        constexpr unsigned short E = T == SPTMM_X_F16 ? 0x7c00 : 0x7f80;
+        return __ballot(most[0] >= E || most[1] >= E) != 0;
     }
 
-    __device__ __forceinline__ u16x8 v_frag(const char *v, int d, int s) const
+    // V for the 32 values of d from 32 b on: for step t the keys 16 t + 4 half + {0..3} and + 8, which are those of this lane's P
+    __device__ __forceinline__ void v_frags(const char *v, int b, u16x8 (&f)[2 * KB]) const
     {
-        // keys 16 s + 4 half + {0..3} and + 8: what this lane holds of P for step s
         typedef __attribute__((address_space(3))) s16x4 *lds4;
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v + v_at[d] + s * 16 * DP * 2));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v + v_at[d] + (s * 16 + 8) * DP * 2));
-        return __builtin_bit_cast(u16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int t = 0; t < 2 * KB; ++t) {
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v + v_at[b] + t * 16 * DP * 2));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v + v_at[b] + (t * 16 + 8) * DP * 2));
+            f[t] = __builtin_bit_cast(u16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
     }
 
     // One tile of keys, from j0 on.  CLEAN: every row of this wavefront sees all of it; EDGE: some do not.  bad: see `polluted`.
-    template <int KIND> __device__ __forceinline__ void step(const AttnParams &p, const char *k, const char *v, int j0, bool bad = false)
+    template <int KIND> __device__ __forceinline__ void step(const AttnParams &p, const char *k, const char *v, int j0 = 0, int lo = 0, bool bad = false)
     {
         const int half = (threadIdx.x & 63) >> 5;
         f32x16 s[KB];
@@ -229,7 +287,7 @@ template <int T, int DP, int KT> struct Rows {
 #pragma unroll
             for (int b = 0; b < KB; ++b)
                 s[b] = mfma<T>(*reinterpret_cast<const u16x8 *>(k + (k_at ^ (ks << 5)) + b * 32 * DP * 2), qf[ks], s[b]);
-        if (KIND != CLEAN) {
+        if (KIND == EDGE && j0 + KT - 1 > lo) {
             const int last = lim - j0 - 4 * half;
 #pragma unroll
             for (int b = 0; b < KB; ++b)
@@ -265,26 +323,30 @@ template <int T, int DP, int KT> struct Rows {
         if (KIND == EDGE && bad) {
             const f32x16 zero = {0.f};
 #pragma unroll
-            for (int t = 0; t < 2 * KB; ++t)
+            for (int d = 0; d < DS; ++d) {
+                u16x8 vf[2 * KB];
+                v_frags(v, d, vf);
+#pragma unroll
+                for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll 1
-                for (int x = 0; x < 16; ++x) {  // element x % 8 of the lower (x < 8) or the upper lanes' eight keys of step t
-                    const int e = x & 7, key = j0 + 16 * t + (e < 4 ? e : e + 4) + 4 * (x >> 3);
-                    u32x4 only;
+                    for (int x = 0; x < 16; ++x) {  // element x % 8 of the lower (x < 8) or the upper lanes' eight keys of step t
+                        const int e = x & 7, key = j0 + 16 * t + (e < 4 ? e : e + 4) + 4 * (x >> 3);
+                        u32x4 only;
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) only[w] = half == x >> 3 && w == e >> 1 ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
-                    const u16x8 one = __builtin_bit_cast(u16x8, __builtin_bit_cast(u32x4, pf[t]) & only);
-#pragma unroll
-                    for (int d = 0; d < DS; ++d) {
-                        const f32x16 n = mfma<T>(__builtin_bit_cast(u16x8, __builtin_bit_cast(u32x4, v_frag(v, d, t)) & only), one, zero);
+                        for (int w = 0; w < 4; ++w) only[w] = half == x >> 3 && w == e >> 1 ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+                        const f32x16 n = mfma<T>(__builtin_bit_cast(u16x8, __builtin_bit_cast(u32x4, vf[t]) & only), __builtin_bit_cast(u16x8, __builtin_bit_cast(u32x4, pf[t]) & only), zero);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[d][i] += key <= lim ? n[i] : 0.f;
                     }
-                }
+            }
         } else {
 #pragma unroll
-            for (int d = 0; d < DS; ++d)
+            for (int d = 0; d < DS; ++d) {
+                u16x8 vf[2 * KB];
+                v_frags(v, d, vf);
 #pragma unroll
-                for (int t = 0; t < 2 * KB; ++t) o[d] = mfma<T>(v_frag(v, d, t), pf[t], o[d]);
+                for (int t = 0; t < 2 * KB; ++t) o[d] = mfma<T>(vf[t], pf[t], o[d]);
+            }
         }
     }
 };
@@ -309,22 +371,17 @@ template <int T> __device__ __forceinline__ void write4(const AttnParams &p, con
 template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) attention_tile_kernel(const AttnParams p)
 {
     static_assert(WAVES == 4, "128 rows");
-    constexpr int LOG_TM = 7;
+    constexpr int LOG_TM = 7, TM = 1 << LOG_TM;
     __shared__ __attribute__((aligned(1024))) char k_a[KT * DP * 2], k_b[KT * DP * 2], v_a[KT * DP * 2], v_b[KT * DP * 2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Tile t;
-    if (!find_tile<LOG_TM>(p, p.slots - 1 - (int)blockIdx.x, &t)) return;  // the longest rows first
-    const int kv_head = blockIdx.y, split = blockIdx.z;
-    const int i_last = (min(t.row0 + 128, t.rows) - 1) / p.group, all = min(t.nk, t.nk - t.nq + i_last + 1);
+    // the rows that see the most keys first, and of all heads before the next rows: workgroups dispatched late are short
+    const int kv_head = (int)(blockIdx.x % (unsigned)p.kv_heads), split = blockIdx.z, rank = (int)(blockIdx.x / (unsigned)p.kv_heads);
+    if (p.batch <= BY_WORK ? !find_tile_by_work<LOG_TM>(p, rank, &t) : !find_tile<LOG_TM>(p, p.slots - 1 - rank, &t)) return;
+    const int i_last = (min(t.row0 + TM, t.rows) - 1) / p.group, all = min(t.nk, t.nk - t.nq + i_last + 1);
     const int begin = split * p.chunk, end = split == p.splits - 1 ? all : min(all, begin + p.chunk);
     if (split && begin >= end) return;
 
-    Rows<T, DP, KT> r;
-    const int row = t.row0 + wave * 32 + (lane & 31);
-    const bool valid = row < t.rows;
-    r.init(p, t, kv_head, valid ? row : t.rows - 1, valid);
-    const int row_w = t.row0 + wave * 32, lo = t.nk - t.nq + row_w / p.group;
-    const int hi = row_w < t.rows ? t.nk - t.nq + min(i_last, (row_w + 31) / p.group) : -1;
     Loader<DP, KT, WAVES> lk, lv;
     lk.init(p.k_stride, p.dim, wave, false);
     lv.init(p.v_stride, p.dim, wave, true);
@@ -334,33 +391,38 @@ template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64
     // tiles that every row of the workgroup sees whole, in pairs: the two pairs of buffers alternate by name, so that the compiler
     // knows which loads a read has to wait for
     const int clean = max(0, min(t.nk - t.nq + t.row0 / p.group + 1, end) - begin) / KT & ~1;
-    auto load = [&](int i, char *kl, char *vl) {
-        if (i >= n) return;
+    auto load = [&](int i, char *kl, char *vl) {  // behind the last tile: zeros, without an access to memory
         const int j = begin + i * KT;
         lk.issue(k + (int64_t)j * p.k_stride, p.k_stride, p.dim, end - j, kl, wave);
         lv.issue(v + (int64_t)j * p.v_stride, p.v_stride, p.dim, end - j, vl, wave);
     };
-    typedef Rows<T, DP, KT> R;
     load(0, k_a, v_a);
+    typedef Rows<T, DP, KT> R;
+    R r;
+    const int row = t.row0 + wave * 32 + (lane & 31);
+    const bool valid = row < t.rows;
+    r.init(p, t, kv_head, valid ? row : t.rows - 1, valid);
+    const int row_w = t.row0 + wave * 32, lo = t.nk - t.nq + row_w / p.group;
+    const int hi = row_w < t.rows ? t.nk - t.nq + min(i_last, (row_w + 31) / p.group) : -1;
     int i = 0;
     for (; i < clean; i += 2) {
         lds_arrived();
         load(i + 1, k_b, v_b);
-        r.template step<R::CLEAN>(p, k_a, v_a, 0);
+        r.template step<R::CLEAN>(p, k_a, v_a);
         lds_arrived();
         load(i + 2, k_a, v_a);
-        r.template step<R::CLEAN>(p, k_b, v_b, 0);
+        r.template step<R::CLEAN>(p, k_b, v_b);
     }
     for (; i < n; ++i) {
         int j = begin + i * KT;
         lds_arrived();
         load(i + 1, k_b, v_b);
-        if (j <= hi) r.template step<R::EDGE>(p, k_a, v_a, j, r.polluted(v_a, j, end, lo));
+        if (j <= hi) r.template step<R::EDGE>(p, k_a, v_a, j, lo, r.polluted(v_a, j, end, lo));
         if (++i >= n) break;
         j += KT;
         lds_arrived();
         load(i + 1, k_a, v_a);
-        if (j <= hi) r.template step<R::EDGE>(p, k_b, v_b, j, r.polluted(v_b, j, end, lo));
+        if (j <= hi) r.template step<R::EDGE>(p, k_b, v_b, j, lo, r.polluted(v_b, j, end, lo));
     }
     const float sum = halves_sum(r.sum), f = p.splits > 1 ? 1.f : 1.f / sum;
     if (!valid) return;
@@ -424,18 +486,18 @@ template <int T, int DP, int WAVES> __global__ void __launch_bounds__(64 * WAVES
     int i = 0;
     for (; i < clean; i += 2) {
         load(i + 1, k_b, v_b);
-        r.template step<R::CLEAN>(p, ka, va, 0);
+        r.template step<R::CLEAN>(p, ka, va);
         load(i + 2, k_a, v_a);
-        r.template step<R::CLEAN>(p, kb, vb, 0);
+        r.template step<R::CLEAN>(p, kb, vb);
     }
     for (; i < n; ++i) {
         int j = j0 + i * STRIDE;
         load(i + 1, k_b, v_b);
-        r.template step<R::EDGE>(p, ka, va, j, r.polluted(va, j, end, lo));
+        r.template step<R::EDGE>(p, ka, va, j, lo, r.polluted(va, j, end, lo));
         if (++i >= n) break;
         j += STRIDE;
         load(i + 1, k_a, v_a);
-        r.template step<R::EDGE>(p, kb, vb, j, r.polluted(vb, j, end, lo));
+        r.template step<R::EDGE>(p, kb, vb, j, lo, r.polluted(vb, j, end, lo));
     }
     // the wavefronts' sums, brought to one maximum and added in wavefront order; a wavefront's part lies where its tiles lay
     const float sum = halves_sum(r.sum);
@@ -560,7 +622,8 @@ int check(const sptmm_attention_args *a)
         return fail(SPTMM_ERR_INVALID, "q_heads must be a positive multiple of kv_heads, at most 65535");
     if (a->head_dim < 8 || a->head_dim > 256 || a->head_dim % 8) return fail(SPTMM_ERR_INVALID, "head_dim must be a multiple of 8, 8..256");
     if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail(SPTMM_ERR_INVALID, "scale must be positive and finite");
-    if ((int64_t)a->total_q * a->q_heads > 0x7fffffff - 256 || (int64_t)a->batch > (1 << 24)) return fail(SPTMM_ERR_INVALID, "total_q * q_heads must stay below 2^31, batch at most 2^24");
+    if ((int64_t)a->total_q * a->q_heads > 0x7fffffff - 256 || (int64_t)a->batch * a->kv_heads > (1 << 22))
+        return fail(SPTMM_ERR_INVALID, "total_q * q_heads must stay below 2^31, batch * kv_heads at most 2^22");
     if (a->kv_rows > (1 << 30)) return fail(SPTMM_ERR_INVALID, "kv_rows must be at most 2^30");
     return SPTMM_OK;
 }
@@ -600,7 +663,7 @@ size_t workspace(const sptmm_attention_args *a, const Cut &c)
 
 template <int T> void launch(const AttnParams &p, const Cut &c, hipStream_t st)
 {
-    const dim3 grid(c.slots, p.kv_heads, c.splits);
+    const dim3 grid = c.keys ? dim3(c.slots, p.kv_heads, c.splits) : dim3(c.slots * p.kv_heads, 1, c.splits);
     if (c.keys) {
         if (c.dp == 64) hipLaunchKernelGGL((attention_keys_kernel<T, 64, 4>), grid, dim3(256), 0, st, p);
         else if (c.dp == 128) hipLaunchKernelGGL((attention_keys_kernel<T, 128, 4>), grid, dim3(256), 0, st, p);
