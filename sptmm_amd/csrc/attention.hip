@@ -92,30 +92,44 @@ struct Tile {
     int q0, nq, k0, nk, row0, rows;  // first query, queries, first cache row, keys; first row of the tile, rows of the sequence
 };
 
+// A sequence's arrays, read by one lane and cut to the buffers
+struct Seq {
+    int q0, nq, k0, nk;
+};
+__device__ __forceinline__ Seq sequence(const AttnParams &p, int b)
+{
+    const int a = p.q_start[b], e = p.q_start[b + 1], at = p.kv_start ? p.kv_start[b] : a, len = p.kv_len ? p.kv_len[b] : e - a;
+    Seq s;
+    s.q0 = min(max(a, 0), p.total_q);
+    s.nq = max(min(max(e, 0), p.total_q) - s.q0, 0);
+    const bool there = at >= 0 && at < p.kv_rows;
+    s.k0 = there ? at : 0;
+    s.nk = there ? (int)min((int64_t)max(len, 0), p.kv_rows - at) : 0;
+    return s;
+}
+
 template <int LOG_TM> __device__ __forceinline__ bool find_tile(const AttnParams &p, int slot, Tile *t)
 {
     const int lane = threadIdx.x & 63;
-    int count = 0;
+    bool found = false;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
         const int b = b0 + lane;
-        bool in = false;
-        if (b < p.batch) in = (int)(((int64_t)min(max(p.q_start[b], 0), p.total_q) * p.group) >> LOG_TM) + b <= slot;
-        count += __popcll(__ballot(in));
+        const Seq s = sequence(p, min(b, p.batch - 1));
+        const int first = (int)(((int64_t)s.q0 * p.group) >> LOG_TM) + b;
+        const int c = __popcll(__ballot(b < p.batch && first <= slot));
+        if (c == 0) break;
+        found = true;
+        t->q0 = __builtin_amdgcn_readlane(s.q0, c - 1);
+        t->nq = __builtin_amdgcn_readlane(s.nq, c - 1);
+        t->k0 = __builtin_amdgcn_readlane(s.k0, c - 1);
+        t->nk = __builtin_amdgcn_readlane(s.nk, c - 1);
+        t->row0 = slot - __builtin_amdgcn_readlane(first, c - 1);
+        if (c < 64) break;
     }
-    const int b = __builtin_amdgcn_readfirstlane(count) - 1;
-    if (b < 0) return false;
-    const int q0 = min(max(p.q_start[b], 0), p.total_q), q1 = min(max(p.q_start[b + 1], 0), p.total_q);
-    t->q0 = q0;
-    t->nq = max(q1 - q0, 0);
+    if (!found || t->row0 > t->nq * p.group >> LOG_TM) return false;
     t->rows = t->nq * p.group;
-    t->row0 = (slot - ((int)(((int64_t)q0 * p.group) >> LOG_TM) + b)) << LOG_TM;
-    if (t->row0 < 0 || t->row0 >= t->rows) return false;
-    const int k0 = p.kv_start ? p.kv_start[b] : q0;
-    int nk = p.kv_len ? p.kv_len[b] : t->nq;
-    if (k0 < 0 || k0 >= p.kv_rows) nk = 0;
-    t->k0 = nk > 0 ? k0 : 0;
-    t->nk = (int)min((int64_t)max(nk, 0), p.kv_rows - t->k0);
-    return true;
+    t->row0 <<= LOG_TM;
+    return t->row0 >= 0 && t->row0 < t->rows;
 }
 
 // The same in the order of the tiles' last keys, the furthest first, over all sequences: a tile's work is proportional to the keys it
@@ -125,15 +139,10 @@ template <int LOG_TM> __device__ __forceinline__ bool find_tile(const AttnParams
 constexpr int BY_WORK = 32;  // sequences, at most (the evaluation walks them)
 template <int LOG_TM> __device__ __forceinline__ bool find_tile_by_work(const AttnParams &p, int rank, Tile *t)
 {
-    const int lane = threadIdx.x & 63, b = min(lane, p.batch - 1);
-    const int q0 = min(max(p.q_start[b], 0), p.total_q), q1 = min(max(p.q_start[b + 1], 0), p.total_q), nq = max(q1 - q0, 0);
-    const int k0 = p.kv_start ? p.kv_start[b] : q0;
-    int nk = p.kv_len ? p.kv_len[b] : nq;
-    if (k0 < 0 || k0 >= p.kv_rows) nk = 0;
-    const int first = nk > 0 ? k0 : 0;
-    nk = (int)min((int64_t)max(nk, 0), p.kv_rows - first);
-    const int tiles = lane < p.batch ? (int)(((int64_t)nq * p.group + (1 << LOG_TM) - 1) >> LOG_TM) : 0;
-    const int off = (int)(((int64_t)(nk - nq) * p.group) >> LOG_TM), behind = off + tiles;
+    const int lane = threadIdx.x & 63;
+    const Seq s = sequence(p, min(lane, p.batch - 1));
+    const int tiles = lane < p.batch ? (int)(((int64_t)s.nq * p.group + (1 << LOG_TM) - 1) >> LOG_TM) : 0;
+    const int off = (int)(((int64_t)(s.nk - s.nq) * p.group) >> LOG_TM), behind = off + tiles;
     int lo = 0x7fffffff, hi = -0x7fffffff;
     for (int i = 0; i < p.batch; ++i)
         if (__builtin_amdgcn_readlane(tiles, i) > 0) {
@@ -158,10 +167,10 @@ template <int LOG_TM> __device__ __forceinline__ bool find_tile_by_work(const At
     unsigned long long who = __ballot(lane < p.batch && off <= place && place < behind);
     for (int r = rank - (have - __popcll(who)); r > 0; --r) who &= who - 1;
     const int seq = __builtin_amdgcn_readfirstlane(__builtin_ctzll(who));
-    t->q0 = __builtin_amdgcn_readlane(q0, seq);
-    t->nq = __builtin_amdgcn_readlane(nq, seq);
-    t->k0 = __builtin_amdgcn_readlane(first, seq);
-    t->nk = __builtin_amdgcn_readlane(nk, seq);
+    t->q0 = __builtin_amdgcn_readlane(s.q0, seq);
+    t->nq = __builtin_amdgcn_readlane(s.nq, seq);
+    t->k0 = __builtin_amdgcn_readlane(s.k0, seq);
+    t->nk = __builtin_amdgcn_readlane(s.nk, seq);
     t->rows = t->nq * p.group;
     t->row0 = (place - __builtin_amdgcn_readlane(off, seq)) << LOG_TM;
     return true;
@@ -177,8 +186,9 @@ template <int DP> __device__ __forceinline__ int swizzle_v(int row) { return DP 
 typedef __attribute__((address_space(3))) void *lds_ptr;
 
 // Rows straight from memory into the LDS: one instruction of a wavefront moves 64 pieces (1 KiB).  Pieces behind the last
-// row or behind the head's last element lie outside the buffer that the descriptor names and arrive as zeros.
-template <int DP, int KT, int WAVES> struct Loader {
+// row or behind the head's last element lie outside the buffer that the descriptor names and arrive as zeros.  STREAM: loads that
+// do not stay in the caches.
+template <int DP, int KT, int WAVES, bool STREAM = false> struct Loader {
     static constexpr int PIECES = DP / 8, PER = KT * PIECES / 64 / WAVES;
     static_assert(PER >= 1, "every wavefront loads something");
     int off[PER];
@@ -199,7 +209,7 @@ template <int DP, int KT, int WAVES> struct Loader {
         const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, bytes, 0x00020000);
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + (i * WAVES + wave) * 1024), 16, off[i], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + (i * WAVES + wave) * 1024), 16, off[i], 0, 0, STREAM ? 2 : 0);
 #endif
     }
 };
@@ -444,7 +454,7 @@ template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64
 }
 
 // ------------------------------------------------------------------------------------------------ KEYS: keys over wavefronts
-template <int T, int DP, int WAVES> __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) attention_keys_kernel(const AttnParams p)
+template <int T, int DP, int WAVES, bool STREAM> __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) attention_keys_kernel(const AttnParams p)
 {
     constexpr int KT = 32, LOG_TM = 5, ONE = KT * DP * 2;
     __shared__ __attribute__((aligned(1024))) char k_a[WAVES * ONE], k_b[WAVES * ONE], v_a[WAVES * ONE], v_b[WAVES * ONE];
@@ -457,25 +467,21 @@ template <int T, int DP, int WAVES> __global__ void __launch_bounds__(64 * WAVES
     const int begin = split * p.chunk, end = split == p.splits - 1 ? all : min(all, begin + p.chunk);
     if (split && begin >= end) return;
 
-    Rows<T, DP, KT> r;
-    const bool valid = (lane & 31) < rows;
-    r.init(p, t, kv_head, t.row0 + (valid ? lane & 31 : 0), valid);
-    const int lo = t.nk - t.nq + t.row0 / p.group;
-    Loader<DP, KT, 1> lk, lv;
+    Loader<DP, KT, 1, STREAM> lk, lv;
     lk.init(p.k_stride, p.dim, 0, false);
     lv.init(p.v_stride, p.dim, 0, true);
     const u16 *k = p.k + (int64_t)t.k0 * p.k_stride + (int64_t)kv_head * p.dim, *v = p.v + (int64_t)t.k0 * p.v_stride + (int64_t)kv_head * p.dim;
     // this wavefront's tiles: every WAVES-th, one in use while the next is on its way
     constexpr int STRIDE = WAVES * KT;
     const int j0 = begin + wave * KT, n = j0 < end ? (end - j0 + STRIDE - 1) / STRIDE : 0;
-    const int whole = min(lo + 1, end) - j0, clean = (whole < KT ? 0 : (whole - KT) / STRIDE + 1) & ~1;
+    const int lo = t.nk - t.nq + t.row0 / p.group, whole = min(lo + 1, end) - j0, clean = (whole < KT ? 0 : (whole - KT) / STRIDE + 1) & ~1;
     auto load = [&](int i, char *kl, char *vl) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the tile that this load overwrites are done
         if (i < n) {
             const int j = j0 + i * STRIDE;
             lk.issue(k + (int64_t)j * p.k_stride, p.k_stride, p.dim, end - j, kl + wave * ONE, 0);
             lv.issue(v + (int64_t)j * p.v_stride, p.v_stride, p.dim, end - j, vl + wave * ONE, 0);
-            if (i) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Loader<DP, KT, 1>::PER) : "memory");  // the tile before this one has landed
+            if (i) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Loader<DP, KT, 1, STREAM>::PER) : "memory");  // the tile before this one has landed
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
@@ -483,6 +489,9 @@ template <int T, int DP, int WAVES> __global__ void __launch_bounds__(64 * WAVES
     typedef Rows<T, DP, KT> R;
     char *const ka = k_a + wave * ONE, *const kb = k_b + wave * ONE, *const va = v_a + wave * ONE, *const vb = v_b + wave * ONE;
     load(0, k_a, v_a);
+    R r;
+    const bool valid = (lane & 31) < rows;
+    r.init(p, t, kv_head, t.row0 + (valid ? lane & 31 : 0), valid);
     int i = 0;
     for (; i < clean; i += 2) {
         load(i + 1, k_b, v_b);
@@ -547,27 +556,25 @@ template <int T, int DP, int WAVES> __global__ void __launch_bounds__(64 * WAVES
 }
 
 // ------------------------------------------------------------------------------------------------ splits joined
-// One wavefront per (query, head): the splits that hold keys the row sees, in their order.
+// One workgroup per (query, head): the splits that hold keys the row sees, shared by its wavefronts, added in a fixed order.
 template <int T> __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), all = (int64_t)p.total_q * p.q_heads;
-    if (row >= all) return;
+    __shared__ __attribute__((aligned(16))) f32x4 parts[4][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = blockIdx.x, all = (int64_t)p.total_q * p.q_heads;
     const int query = (int)(row / p.q_heads), head = (int)(row - (int64_t)query * p.q_heads);
     // the sequence of this query: the last one that starts at or before it
-    int count = 0;
+    Seq s = {0, 0, 0, 0};
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
         const int b = b0 + lane;
-        count += __popcll(__ballot(b < p.batch && min(max(p.q_start[b], 0), p.total_q) <= query));
+        const Seq mine = sequence(p, min(b, p.batch - 1));
+        const int c = __popcll(__ballot(b < p.batch && mine.q0 <= query));
+        if (c == 0) break;
+        s = {__builtin_amdgcn_readlane(mine.q0, c - 1), __builtin_amdgcn_readlane(mine.nq, c - 1), 0, __builtin_amdgcn_readlane(mine.nk, c - 1)};
+        if (c < 64) break;
     }
-    const int b = __builtin_amdgcn_readfirstlane(count) - 1;
-    if (b < 0) return;
-    const int q0 = min(max(p.q_start[b], 0), p.total_q), q1 = min(max(p.q_start[b + 1], 0), p.total_q);
-    if (query >= q1) return;  // a row behind the last sequence
-    const int k0 = p.kv_start ? p.kv_start[b] : q0;
-    int64_t nk = p.kv_len ? p.kv_len[b] : q1 - q0;
-    nk = k0 < 0 || k0 >= p.kv_rows ? 0 : min(max(nk, (int64_t)0), p.kv_rows - k0);
-    const int seen = (int)nk - (q1 - q0) + (query - q0) + 1;
+    if (query >= s.q0 + s.nq) return;  // a row behind the last sequence
+    const int seen = s.nk - s.nq + (query - s.q0) + 1;
     const int n = seen <= 0 ? 0 : min(p.splits, (seen + p.chunk - 1) / p.chunk);
     // every lane holds the weight of one split (and of those 64, 128 and 192 further)
     float2 ml[4];
@@ -587,30 +594,41 @@ template <int T> __global__ void __launch_bounds__(256) attention_join_kernel(co
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-    // four values a lane, and as many splits side by side as lanes are left
+    // four values a lane, and as many splits side by side as lanes are left, and every fourth such group a wavefront's
+    constexpr int WAVES = 4;
     const int quads = p.dim / 4, log_l = quads <= 2 ? 1 : 32 - __builtin_clz(quads - 1), sub = lane >> log_l, d4 = lane & ((1 << log_l) - 1), step = 64 >> log_l;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if (64 * i >= n) break;
-        for (int s0 = 64 * i; s0 < min(n, 64 * i + 64); s0 += step) {
-            const int s = s0 + sub;
-            const float f = __shfl(w[i], s & 63, 64);
-            if (s < n && d4 < quads) {
-                const f32x4 x = *reinterpret_cast<const f32x4 *>(p.part_o + (s * all + row) * p.dim + 4 * d4);
+        const int end = min(64, n - 64 * i);
+        for (int s0 = wave * step; s0 < end; s0 += 4 * WAVES * step) {
+            f32x4 x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+            for (int u = 0; u < 4; ++u) {  // (four loads in flight; behind the last split: its values, times zero)
+                const int at = min(64 * i + s0 + u * WAVES * step + sub, n - 1);
+                x[u] = *reinterpret_cast<const f32x4 *>(p.part_o + (at * all + row) * p.dim + 4 * min(d4, quads - 1));
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int at = s0 + u * WAVES * step + sub;
+                const float f = __shfl(w[i], at & 63, 64);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = at < end ? fmaf(x[u][e], f, o[e]) : o[e];
             }
         }
     }
     for (int l = 1 << log_l; l < 64; l <<= 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], l, 64);
+    parts[wave][lane] = o;
+    __syncthreads();
+    if (wave || sub || d4 >= quads) return;
+    o = (parts[0][lane] + parts[1][lane]) + (parts[2][lane] + parts[3][lane]);
     const float inv = 1.f / sum;
     u16x4 y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = narrow<T>(n ? o[e] * inv : 0.f);
-    if (sub == 0 && d4 < quads) *reinterpret_cast<u16x4 *>(p.out + (int64_t)query * p.out_stride + (int64_t)head * p.dim + 4 * d4) = y;
+    *reinterpret_cast<u16x4 *>(p.out + (int64_t)query * p.out_stride + (int64_t)head * p.dim + 4 * d4) = y;
 }
 
 int check(const sptmm_attention_args *a)
@@ -631,6 +649,7 @@ int check(const sptmm_attention_args *a)
 // how a call is cut up: by its sizes alone
 struct Cut {
     bool keys;  // the KEYS form
+    bool stream;
     int dp, slots, splits, chunk;
 };
 
@@ -651,6 +670,7 @@ Cut cut(const sptmm_attention_args *a)
     c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
     c.chunk = std::max(unit, (max_kv / c.splits + 127) / 128 * 128);
     c.splits = std::max(1, std::min(c.splits, (max_kv + c.chunk - 1) / c.chunk));
+    c.stream = (int64_t)a->batch * max_kv * a->kv_heads * a->head_dim * 4 > (128ll << 20);
     return c;
 }
 
@@ -665,16 +685,17 @@ template <int T> void launch(const AttnParams &p, const Cut &c, hipStream_t st)
 {
     const dim3 grid = c.keys ? dim3(c.slots, p.kv_heads, c.splits) : dim3(c.slots * p.kv_heads, 1, c.splits);
     if (c.keys) {
-        if (c.dp == 64) hipLaunchKernelGGL((attention_keys_kernel<T, 64, 4>), grid, dim3(256), 0, st, p);
-        else if (c.dp == 128) hipLaunchKernelGGL((attention_keys_kernel<T, 128, 4>), grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((attention_keys_kernel<T, 256, 2>), grid, dim3(128), 0, st, p);
+        const auto kernel = c.dp == 64    ? (c.stream ? attention_keys_kernel<T, 64, 2, true> : attention_keys_kernel<T, 64, 2, false>)
+                            : c.dp == 128 ? (c.stream ? attention_keys_kernel<T, 128, 2, true> : attention_keys_kernel<T, 128, 2, false>)
+                                          : (c.stream ? attention_keys_kernel<T, 256, 2, true> : attention_keys_kernel<T, 256, 2, false>);
+        hipLaunchKernelGGL(kernel, grid, dim3(128), 0, st, p);
     } else {
         if (c.dp == 64) hipLaunchKernelGGL((attention_tile_kernel<T, 64, 64, 4>), grid, dim3(256), 0, st, p);
         else if (c.dp == 128) hipLaunchKernelGGL((attention_tile_kernel<T, 128, 64, 4>), grid, dim3(256), 0, st, p);
         else hipLaunchKernelGGL((attention_tile_kernel<T, 256, 32, 4>), grid, dim3(256), 0, st, p);
     }
     if (c.splits > 1)
-        hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)(((int64_t)p.total_q * p.q_heads + 3) / 4)), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)((int64_t)p.total_q * p.q_heads)), dim3(256), 0, st, p);
 }
 
 }  // namespace
@@ -712,7 +733,8 @@ extern "C" int sptmm_attention(const sptmm_attention_args *a, void *workspace_de
     p.c = a->scale * 1.44269504088896340736f;
     p.slots = c.slots, p.splits = c.splits, p.chunk = c.chunk;
     p.part_o = (float *)workspace_dev;
-    p.part_ml = want ? (float2 *)((char *)workspace_dev + ((size_t)a->total_q * a->q_heads * c.splits * a->head_dim * 4 + 255) / 256 * 256) : nullptr;
+    const size_t o_bytes = ((size_t)a->total_q * a->q_heads * c.splits * a->head_dim * 4 + 255) / 256 * 256;
+    p.part_ml = want ? (float2 *)((char *)workspace_dev + o_bytes) : nullptr;
     a->type == SPTMM_X_F16 ? launch<SPTMM_X_F16>(p, c, (hipStream_t)stream) : launch<SPTMM_X_BF16>(p, c, (hipStream_t)stream);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? SPTMM_OK : fail(SPTMM_ERR_HIP, "attention kernels launch: %s (%d)", hipGetErrorString(e), (int)e);
