@@ -385,8 +385,14 @@ template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64
     __shared__ __attribute__((aligned(1024))) char k_a[KT * DP * 2], k_b[KT * DP * 2], v_a[KT * DP * 2], v_b[KT * DP * 2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Tile t;
-    // the rows that see the most keys first, and of all heads before the next rows: workgroups dispatched late are short
-    const int kv_head = (int)(blockIdx.x % (unsigned)p.kv_heads), split = blockIdx.z, rank = (int)(blockIdx.x / (unsigned)p.kv_heads);
+    // The rows that see the most keys first, and of all heads before the next rows: workgroups dispatched late are short.
+    // Workgroups go to the eight XCDs in turn, and those that read the same head's keys should share an L2: without splits the
+    // tiles are dealt into eight hands, and each XCD takes as many neighbouring hands as there are heads, of at most two or
+    // three heads then (one prompt of 8192 tokens, 5 heads: a fifth of the reads that miss L2).  With splits the heads' parts
+    // differ in work by split, and are spread as they come.
+    const unsigned heads = (unsigned)p.kv_heads;
+    const unsigned x = blockIdx.x, hand = x % 8 * heads + x / 8 % heads;
+    const int kv_head = (int)(p.splits > 1 ? x % heads : hand / 8), split = blockIdx.z, rank = (int)(p.splits > 1 ? x / heads : x / 8 / heads * 8 + hand % 8);
     if (p.batch <= BY_WORK ? !find_tile_by_work<LOG_TM>(p, rank, &t) : !find_tile<LOG_TM>(p, p.slots - 1 - rank, &t)) return;
     const int i_last = (min(t.row0 + TM, t.rows) - 1) / p.group, all = min(t.nk, t.nk - t.nq + i_last + 1);
     const int begin = split * p.chunk, end = split == p.splits - 1 ? all : min(all, begin + p.chunk);
@@ -556,12 +562,15 @@ template <int T, int DP, int WAVES, bool STREAM> __global__ void __launch_bounds
 }
 
 // ------------------------------------------------------------------------------------------------ splits joined
-// One workgroup per (query, head): the splits that hold keys the row sees, shared by its wavefronts, added in a fixed order.
-template <int T> __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
+// Per (query, head) the splits that hold keys the row sees, added in a fixed order, by WAVES wavefronts: the four of a workgroup
+// where there are many splits (one row of 63: 13 us by a single wavefront, 4 by four), one where there are few and many
+// rows (870 x 20 rows of four: 33 us by four wavefronts each, 18 by one).
+template <int T, int WAVES> __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
 {
     __shared__ __attribute__((aligned(16))) f32x4 parts[4][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = blockIdx.x, all = (int64_t)p.total_q * p.q_heads;
+    const int lane = threadIdx.x & 63, in_block = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = WAVES == 1 ? 0 : in_block;
+    const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + in_block : blockIdx.x, all = (int64_t)p.total_q * p.q_heads;
+    if (row >= all) return;
     const int query = (int)(row / p.q_heads), head = (int)(row - (int64_t)query * p.q_heads);
     // the sequence of this query: the last one that starts at or before it
     Seq s = {0, 0, 0, 0};
@@ -594,8 +603,7 @@ template <int T> __global__ void __launch_bounds__(256) attention_join_kernel(co
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-    // four values a lane, and as many splits side by side as lanes are left, and every fourth such group a wavefront's
-    constexpr int WAVES = 4;
+    // four values a lane, and as many splits side by side as lanes are left, and every WAVES-th such group a wavefront's
     const int quads = p.dim / 4, log_l = quads <= 2 ? 1 : 32 - __builtin_clz(quads - 1), sub = lane >> log_l, d4 = lane & ((1 << log_l) - 1), step = 64 >> log_l;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -620,10 +628,12 @@ template <int T> __global__ void __launch_bounds__(256) attention_join_kernel(co
     for (int l = 1 << log_l; l < 64; l <<= 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], l, 64);
-    parts[wave][lane] = o;
-    __syncthreads();
+    if constexpr (WAVES == 4) {
+        parts[wave][lane] = o;
+        __syncthreads();
+        o = (parts[0][lane] + parts[1][lane]) + (parts[2][lane] + parts[3][lane]);
+    }
     if (wave || sub || d4 >= quads) return;
-    o = (parts[0][lane] + parts[1][lane]) + (parts[2][lane] + parts[3][lane]);
     const float inv = 1.f / sum;
     u16x4 y;
 #pragma unroll
@@ -662,11 +672,15 @@ Cut cut(const sptmm_attention_args *a)
     const int tm = c.keys ? 32 : 128;
     const int64_t rows = (int64_t)a->total_q * group;
     c.slots = (int)(rows / tm + a->batch);
-    // workgroups without splits (those that have rows): about as many as sequences have tiles
+    // Workgroups without splits (those that have rows): about as many as sequences have tiles.  Splits where they are fewer than
+    // the chip holds -- of the KEYS form at least four per compute unit, of the TILE form two (one for heads of 256) --, yet
+    // three quarters of that in the TILE form: an exact fit leaves some units a third workgroup to do after the others (512 rows against 16000
+    // keys, 8 heads: 384 workgroups 109 us, 512 workgroups 132; four chunks of 130 to 250 tokens against 12000 to 20000: 201 and 190).
     const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>(c.slots, c.keys ? (int64_t)a->batch : rows / tm + 1)) * a->kv_heads;
+    const int64_t room = c.keys ? 512 : c.dp == 256 ? 192 : 384;
     const int max_kv = (int)std::min<int64_t>(a->max_kv, a->kv_rows);
     const int unit = c.keys ? 128 : 512;  // keys a workgroup should have at least
-    const int64_t want = (512 + tiles - 1) / tiles, most = (max_kv + unit - 1) / unit;
+    const int64_t want = (room + tiles - 1) / tiles, most = (max_kv + unit - 1) / unit;
     c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
     c.chunk = std::max(unit, (max_kv / c.splits + 127) / 128 * 128);
     c.splits = std::max(1, std::min(c.splits, (max_kv + c.chunk - 1) / c.chunk));
@@ -683,7 +697,7 @@ size_t workspace(const sptmm_attention_args *a, const Cut &c)
 
 template <int T> void launch(const AttnParams &p, const Cut &c, hipStream_t st)
 {
-    const dim3 grid = c.keys ? dim3(c.slots, p.kv_heads, c.splits) : dim3(c.slots * p.kv_heads, 1, c.splits);
+    const dim3 grid = c.keys ? dim3(c.slots, p.kv_heads, c.splits) : dim3((unsigned)(c.splits > 1 ? c.slots : (c.slots + 7) / 8 * 8) * p.kv_heads, 1, c.splits);
     if (c.keys) {
         const auto kernel = c.dp == 64    ? (c.stream ? attention_keys_kernel<T, 64, 2, true> : attention_keys_kernel<T, 64, 2, false>)
                             : c.dp == 128 ? (c.stream ? attention_keys_kernel<T, 128, 2, true> : attention_keys_kernel<T, 128, 2, false>)
@@ -694,8 +708,9 @@ template <int T> void launch(const AttnParams &p, const Cut &c, hipStream_t st)
         else if (c.dp == 128) hipLaunchKernelGGL((attention_tile_kernel<T, 128, 64, 4>), grid, dim3(256), 0, st, p);
         else hipLaunchKernelGGL((attention_tile_kernel<T, 256, 32, 4>), grid, dim3(256), 0, st, p);
     }
-    if (c.splits > 1)
-        hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)((int64_t)p.total_q * p.q_heads)), dim3(256), 0, st, p);
+    if (c.splits <= 1) return;
+    if (c.splits > 8) hipLaunchKernelGGL((attention_join_kernel<T, 4>), dim3((unsigned)(p.total_q * p.q_heads)), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((attention_join_kernel<T, 1>), dim3((unsigned)((p.total_q * p.q_heads + 3) / 4)), dim3(256), 0, st, p);
 }
 
 }  // namespace
