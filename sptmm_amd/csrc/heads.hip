@@ -13,6 +13,7 @@
 // head of 128 takes 16 lanes and a wavefront handles four heads at a time; the sines of a token's four pairs stay in the
 // lane's registers while it walks the token's heads.
 #include <cmath>
+#include <type_traits>
 
 #include "internal.hpp"
 #include "lanes.hpp"
@@ -22,6 +23,7 @@ namespace {
 
 typedef unsigned short u16;
 typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
+typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 
 struct HeadsParams {
@@ -56,40 +58,48 @@ template <bool INTER> __device__ __forceinline__ int element(const HeadsParams &
     return s < p.pairs ? s + w * p.pairs : 2 * p.pairs + (s - p.pairs) + w * rest;
 }
 
-template <int IN, bool INTER, bool WIDE> __device__ __forceinline__ void load8(const HeadsParams &p, const void *row, int s0, int slots, float (&x)[2][4])
+// a lane's eight elements as they lie in memory
+template <int IN> struct Raw {
+    typedef typename std::conditional<IN == SPTMM_X_F32, f32x4, u16x4>::type Run;
+    typedef typename std::conditional<IN == SPTMM_X_F32, float, u16>::type One;
+    Run a, b;
+    static __device__ __forceinline__ float value(One x)
+    {
+        if constexpr (IN == SPTMM_X_F32) return x;
+        else return widen<IN>(x);
+    }
+};
+
+// four consecutive pair slots from s0 on: two runs of four elements (apart; neighbouring pairs: one run of eight)
+template <int IN, bool INTER, bool WIDE> __device__ __forceinline__ void fetch8(const HeadsParams &p, const void *row, int s0, int slots, Raw<IN> &r)
 {
+    typedef typename Raw<IN>::One One;
+    typedef typename Raw<IN>::Run Run;
+    const One *const x = (const One *)row;
     if constexpr (WIDE) {
-        // four consecutive pair slots: two runs of four elements (apart: two loads; neighbouring pairs: one run of eight)
-        const int e0 = INTER ? 2 * s0 : element<INTER>(p, s0, 0), e1 = INTER ? 2 * s0 + 4 : element<INTER>(p, s0, 1);
-        float r[2][4];
-        if constexpr (IN == SPTMM_X_F32) {
-            const f32x4 a = *reinterpret_cast<const f32x4 *>((const float *)row + e0), b = *reinterpret_cast<const f32x4 *>((const float *)row + e1);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[0][i] = a[i], r[1][i] = b[i];
+        if constexpr (INTER && IN != SPTMM_X_F32) {
+            const u16x8 ab = *reinterpret_cast<const u16x8 *>(x + 2 * s0);
+            r.a = __builtin_shufflevector(ab, ab, 0, 1, 2, 3), r.b = __builtin_shufflevector(ab, ab, 4, 5, 6, 7);
         } else {
-            const u16x4 a = *reinterpret_cast<const u16x4 *>((const u16 *)row + e0), b = *reinterpret_cast<const u16x4 *>((const u16 *)row + e1);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[0][i] = widen<IN>(a[i]), r[1][i] = widen<IN>(b[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[0][i] = INTER ? r[i / 2][2 * (i & 1)] : r[0][i];
-            x[1][i] = INTER ? r[i / 2][2 * (i & 1) + 1] : r[1][i];
+            r.a = *reinterpret_cast<const Run *>(x + (INTER ? 2 * s0 : element<INTER>(p, s0, 0)));
+            r.b = *reinterpret_cast<const Run *>(x + (INTER ? 2 * s0 + 4 : element<INTER>(p, s0, 1)));
         }
     } else {
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
+        for (int i = 0; i < 4; ++i) {
+            // (held as the wide loads would hold them)
+            const int sa = INTER ? s0 + i / 2 : s0 + i, sb = INTER ? s0 + 2 + i / 2 : s0 + i;
+            r.a[i] = sa < slots ? x[element<INTER>(p, sa, INTER ? i & 1 : 0)] : One(0);
+            r.b[i] = sb < slots ? x[element<INTER>(p, sb, INTER ? i & 1 : 1)] : One(0);
+        }
+    }
+}
+template <int IN, bool INTER> __device__ __forceinline__ void unpack8(const Raw<IN> &r, float (&x)[2][4])
+{
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[w][i] = 0.f;
-                if (s0 + i < slots) {
-                    const int e = element<INTER>(p, s0 + i, w);
-                    if constexpr (IN == SPTMM_X_F32)
-                        x[w][i] = ((const float *)row)[e];
-                    else
-                        x[w][i] = widen<IN>(((const u16 *)row)[e]);
-                }
-            }
+    for (int i = 0; i < 4; ++i) {
+        x[0][i] = Raw<IN>::value(INTER ? (i < 2 ? r.a[2 * i] : r.b[2 * i - 4]) : r.a[i]);
+        x[1][i] = Raw<IN>::value(INTER ? (i < 2 ? r.a[2 * i + 1] : r.b[2 * i - 3]) : r.b[i]);
     }
 }
 
@@ -103,8 +113,12 @@ template <int OUT, bool INTER, bool WIDE> __device__ __forceinline__ void store8
             a[i] = narrow<OUT>(INTER ? x[i & 1][i / 2] : x[0][i]);
             b[i] = narrow<OUT>(INTER ? x[i & 1][2 + i / 2] : x[1][i]);
         }
-        *reinterpret_cast<u16x4 *>(row + e0) = a;
-        *reinterpret_cast<u16x4 *>(row + e1) = b;
+        if constexpr (INTER) {
+            *reinterpret_cast<u16x8 *>(row + e0) = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            *reinterpret_cast<u16x4 *>(row + e0) = a;
+            *reinterpret_cast<u16x4 *>(row + e1) = b;
+        }
     } else {
 #pragma unroll
         for (int w = 0; w < 2; ++w)
@@ -114,74 +128,114 @@ template <int OUT, bool INTER, bool WIDE> __device__ __forceinline__ void store8
     }
 }
 
+// Sine and cosine of the angle that position * turns / 2^64 is a fraction of a turn of.  The upper 32 bits of the phase are more
+// than a float holds; the nearest quarter turn is taken off them as an integer, and what is left, an eighth of a turn either
+// way, goes into the Taylor polynomials up to x^9 and x^8 (off by 2^-29 and 2^-25 at the ends).
+__device__ __forceinline__ void turn(int position, unsigned turns_hi, unsigned turns_lo, float &sine, float &cosine)
+{
+    const unsigned pos = (unsigned)position;
+    unsigned phase = pos * turns_hi + __umulhi(pos, turns_lo);
+    if (position < 0) phase -= turns_lo;
+    const unsigned quarter = (phase + 0x20000000u) >> 30;
+    const float x = (float)(int)(phase - (quarter << 30)) * 1.46291807926715968e-9f;  // 2 pi / 2^32
+    const float z = x * x;
+    const float s = x * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 2.75573192e-6f, -1.98412698e-4f), 8.33333333e-3f), -1.66666667e-1f), 1.0f);
+    const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 2.48015873e-5f, -1.38888889e-3f), 4.16666667e-2f), -0.5f), 1.0f);
+    const float a = quarter & 1 ? c : s, b = quarter & 1 ? s : c;
+    sine = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, a) ^ (quarter & 2) << 30);
+    cosine = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, b) ^ ((quarter + 1) & 2) << 30);
+}
+
+constexpr int ROUNDS = 2;  // rounds of heads whose loads a wavefront has in flight together (four take registers that more wavefronts use better)
+
 // IN: type of the rows; OUT: type of the heads written; INTER: pairs of neighbours (2j, 2j+1), else of halves (j, j + pairs);
 // WIDE: every run of four elements lies aligned for one load or store
 template <int IN, int OUT, bool INTER, bool WIDE> __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p)
 {
     const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (unit >= (int64_t)p.tokens * p.parts) return;
-    const int t = (int)(unit / p.parts), part = (int)(unit - (int64_t)t * p.parts);
     const int per_wave = 64 >> p.log_lanes, sub = lane >> p.log_lanes, s0 = (lane & ((1 << p.log_lanes) - 1)) * 4, slots = p.dim / 2;
     const bool mine = s0 < slots;
-    const int first = part * p.per_part, end = min(p.heads, first + p.per_part);
-
-    float cs[4], sn[4];
-    {
-        const int pos = p.positions ? p.positions[t] : t;
+    // the lane's frequencies and gains
+    unsigned t_hi[4], t_lo[4];
+    float gq[2][4], gk[2][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            cs[i] = 1.f, sn[i] = 0.f;
-            if (s0 + i < p.pairs) {
-                // the phase as a signed fraction of a turn: 32 of its 64 bits are more than a float holds
-                const uint64_t phase = (uint64_t)(int64_t)pos * p.turns[s0 + i];
-                const float half_turns = (float)(int)(phase >> 32) * 0x1p-31f;
-                sincospif(half_turns, &sn[i], &cs[i]);
-            }
-        }
+    for (int i = 0; i < 4; ++i) {
+        const uint64_t x = s0 + i < p.pairs ? p.turns[s0 + i] : 0;
+        t_hi[i] = (unsigned)(x >> 32), t_lo[i] = (unsigned)x;
     }
-    int64_t kv_row = p.kv_rows ? p.kv_rows[t] : t;
-    const bool kept = kv_row >= 0 && kv_row < p.kv_capacity;
-
-    constexpr int ESZ = IN == SPTMM_X_F32 ? 4 : 2;
-    for (int h0 = first; h0 < end; h0 += per_wave) {
-        const int h = h0 + sub;
-        const bool is_q = h < p.q_heads, is_v = h >= p.q_heads + p.kv_heads, live = mine && h < end;
-        const int at = is_q ? h : is_v ? h - p.q_heads - p.kv_heads : h - p.q_heads;
-        const char *src = (const char *)(is_q ? p.q : is_v ? p.v : p.k) + ((int64_t)t * (is_q ? p.q_stride : is_v ? p.v_stride : p.k_stride) + (int64_t)at * p.dim) * ESZ;
-        float x[2][4] = {{0.f}};
-        if (live) load8<IN, INTER, WIDE>(p, src, s0, slots, x);
-        const float *gain = is_q ? p.q_gain : p.k_gain;
-        if (gain && !is_v) {  // (lanes of one head agree)
-            float sum = 0.f;
+    {
+        Raw<SPTMM_X_F32> g, h;
+        g.a = g.b = h.a = h.b = f32x4{1.f, 1.f, 1.f, 1.f};
+        if (p.q_gain && mine) fetch8<SPTMM_X_F32, INTER, WIDE>(p, p.q_gain, s0, slots, g);
+        if (p.k_gain && mine) fetch8<SPTMM_X_F32, INTER, WIDE>(p, p.k_gain, s0, slots, h);
+        unpack8<SPTMM_X_F32, INTER>(g, gq);
+        unpack8<SPTMM_X_F32, INTER>(h, gk);
+    }
+    const int64_t units = (int64_t)p.tokens * p.parts;
+    for (int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += (int64_t)gridDim.x * 4) {
+        const int t = p.parts == 1 ? (int)unit : (int)(unit / p.parts), part = (int)(unit - (int64_t)t * p.parts);
+        const int first = part * p.per_part, end = min(p.heads, first + p.per_part);
+        const int pos = p.positions ? p.positions[t] : t;
+        const int64_t kv_row = p.kv_rows ? p.kv_rows[t] : t;
+        const bool kept = kv_row >= 0 && kv_row < p.kv_capacity;
+        constexpr int ESZ = IN == SPTMM_X_F32 ? 4 : 2;
+        float cs[4], sn[4];
+        bool ready = false;
+        for (int h0 = first; h0 < end; h0 += ROUNDS * per_wave) {
+            // the loads of all rounds first
+            Raw<IN> raw[ROUNDS];
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum = fmaf(x[w][i], x[w][i], sum);
-            for (int o = 1; o < 1 << p.log_lanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
-            const float r = 1.0f / sqrtf(fmaf(sum, p.inv_dim, p.eps));
-            if (live) {
-                float g[2][4];
-                load8<SPTMM_X_F32, INTER, WIDE>(p, gain, s0, slots, g);
-#pragma unroll
-                for (int w = 0; w < 2; ++w)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[w][i] = x[w][i] * r * g[w][i];
+            for (int u = 0; u < ROUNDS; ++u) {
+                const int h = h0 + u * per_wave + sub;
+                const bool is_q = h < p.q_heads, is_v = h >= p.q_heads + p.kv_heads;
+                const int at = is_q ? h : is_v ? h - p.q_heads - p.kv_heads : h - p.q_heads;
+                const char *src = (const char *)(is_q ? p.q : is_v ? p.v : p.k) + ((int64_t)t * (is_q ? p.q_stride : is_v ? p.v_stride : p.k_stride) + (int64_t)at * p.dim) * ESZ;
+                if (mine && h < end) fetch8<IN, INTER, WIDE>(p, src, s0, slots, raw[u]);
+                else raw[u].a = raw[u].b = typename Raw<IN>::Run{0, 0, 0, 0};
             }
-        }
-        if (!is_v)
+            if (!ready) {  // the token's sines, while the loads are on their way
+                ready = true;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (s0 + i < p.pairs) {
-                    const float a = x[0][i], b = x[1][i];
-                    x[0][i] = a * cs[i] - b * sn[i];
-                    x[1][i] = b * cs[i] + a * sn[i];
+                for (int i = 0; i < 4; ++i) turn(pos, t_hi[i], t_lo[i], sn[i], cs[i]);
+            }
+#pragma unroll
+            for (int u = 0; u < ROUNDS; ++u) {
+                const int h = h0 + u * per_wave + sub;
+                if (h - sub >= end) break;
+                const bool is_q = h < p.q_heads, is_v = h >= p.q_heads + p.kv_heads;
+                const int at = is_q ? h : is_v ? h - p.q_heads - p.kv_heads : h - p.q_heads;
+                float x[2][4];
+                unpack8<IN, INTER>(raw[u], x);
+                if (p.q_gain || p.k_gain) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int w = 0; w < 2; ++w)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sum = fmaf(x[w][i], x[w][i], sum);
+                    if (p.log_lanes >= 2) sum = lanes_sum(sum, p.log_lanes);
+                    else if (p.log_lanes == 1) sum += dpp<0xB1>(sum);  // quad_perm [1,0,3,2]
+                    if (!is_v && (is_q ? p.q_gain : p.k_gain)) {  // (lanes of one head agree)
+                        const float r = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
+#pragma unroll
+                        for (int w = 0; w < 2; ++w)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) x[w][i] = x[w][i] * r * (is_q ? gq[w][i] : gk[w][i]);
+                    }
+                }
+                if (!is_v)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (s0 + i < p.pairs) {
+                            const float a = x[0][i], b = x[1][i];
+                            x[0][i] = a * cs[i] - b * sn[i];
+                            x[1][i] = b * cs[i] + a * sn[i];
+                        }
+                if (mine && h < end && (is_q || kept)) {
+                    u16 *dst = (u16 *)(is_q ? p.q_out : is_v ? p.v_out : p.k_out) +
+                               ((is_q ? (int64_t)t * p.q_out_stride : kv_row * (is_v ? p.v_out_stride : p.k_out_stride)) + (int64_t)at * p.dim);
+                    store8<OUT, INTER, WIDE>(p, dst, s0, slots, x);
                 }
             }
-        if (live && (is_q || kept)) {
-            u16 *dst = (u16 *)(is_q ? p.q_out : is_v ? p.v_out : p.k_out) +
-                       ((is_q ? (int64_t)t * p.q_out_stride : kv_row * (is_v ? p.v_out_stride : p.k_out_stride)) + (int64_t)at * p.dim);
-            store8<OUT, INTER, WIDE>(p, dst, s0, slots, x);
         }
     }
 }
@@ -267,21 +321,20 @@ extern "C" int sptmm_heads_norm_rotate(const sptmm_heads_args *a, void *stream)
     while ((8 << p.log_lanes) < a->head_dim) ++p.log_lanes;
     const int per_wave = 64 >> p.log_lanes, rounds = (p.heads + per_wave - 1) / per_wave;
     // One wavefront per round of heads while that leaves the chip's wavefront slots unfilled (a lone token: one round of
-    // latency instead of eight), one wavefront per token once there are enough tokens (the sines are computed once).
-    p.parts = a->tokens >= 2048 ? 1 : rounds;
+    // latency instead of eight); one per token once there are enough tokens (its sines are computed once).
+    p.parts = a->tokens >= 1024 ? 1 : rounds;
     const int rounds_per_part = (rounds + p.parts - 1) / p.parts;
     p.per_part = rounds_per_part * per_wave;
     const int64_t units = (int64_t)a->tokens * p.parts;
-    if (units > (int64_t)4 * 0x7fffffff) return fail(SPTMM_ERR_INVALID, "too many tokens");
-    const int blocks = (int)((units + 3) / 4);
+    const int blocks = (int)std::min<int64_t>((units + 3) / 4, 1 << 22);
 
     // runs of four elements aligned for one load / store: in the head (dim, pairs) and from row to row
-    const size_t in4 = 4 * isz;
+    const size_t in4 = inter && isz == 2 ? 16 : 4 * isz, out4 = inter ? 16 : 8;
     bool wide = a->head_dim % 8 == 0 && (inter || p.pairs % 4 == 0);
     const int64_t strides[6] = {a->q_stride, a->k_stride, has_v ? a->v_stride : 0, a->q_out_stride, a->k_out_stride, has_v ? a->v_out_stride : 0};
-    for (int64_t s : strides) wide = wide && s % 4 == 0;
+    for (int64_t s : strides) wide = wide && s % (inter ? 8 : 4) == 0;
     for (const void *x : ins) wide = wide && aligned(x, in4);
-    for (const void *x : outs) wide = wide && aligned(x, 8);
+    for (const void *x : outs) wide = wide && aligned(x, out4);
     wide = wide && aligned(a->q_gain, 16) && aligned(a->k_gain, 16);
 
     hipStream_t st = (hipStream_t)stream;
