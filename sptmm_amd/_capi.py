@@ -88,12 +88,12 @@ class Rotation(C.Structure):
 
 def _dev(x):
     """A device address: a DeviceBuffer's, or an address as it is (None: NULL)."""
-    return x.ptr if isinstance(x, DeviceBuffer) else x
+    return x.ptr if type(x) is DeviceBuffer else x
 
 
 def _stream(s):
     """A Stream's handle, or a hipStream_t as it is (None: the default stream)."""
-    return s.handle if isinstance(s, Stream) else s
+    return s.handle if type(s) is Stream else s
 
 
 class _Args(C.Structure):
@@ -209,10 +209,10 @@ def lib() -> C.CDLL:
         L.sptmm_adapters_free.argtypes = [C.c_void_p]
         L.sptmm_adapters_free.restype = None
         L.sptmm_rotation_init.argtypes = [C.c_void_p, C.c_int, C.c_int, C.POINTER(Rotation)]
-        L.sptmm_heads_norm_rotate.argtypes = [C.POINTER(HeadsArgs), C.c_void_p]
+        L.sptmm_heads_norm_rotate.argtypes = [C.c_void_p, C.c_void_p]  # (an address converts in a third of a reference's time)
         L.sptmm_attention_workspace_bytes.argtypes = [C.POINTER(AttentionArgs)]
         L.sptmm_attention_workspace_bytes.restype = C.c_size_t
-        L.sptmm_attention.argtypes = [C.POINTER(AttentionArgs), C.c_void_p, C.c_size_t, C.c_void_p]
+        L.sptmm_attention.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
         _LIB = L
     return _LIB
 
@@ -581,7 +581,11 @@ def copy_kernel(dst: DeviceBuffer, src: DeviceBuffer, nbytes: int, stream: Strea
 
 def heads_norm_rotate(args: HeadsArgs, stream: "Stream | int | None" = None):
     """Norms of query and key heads, rotation by position, 16-bit heads out, keys and values to their cache rows (one launch)."""
-    _ck(lib().sptmm_heads_norm_rotate(C.byref(args), _stream(stream)))
+    if type(args) is not HeadsArgs:
+        raise TypeError("args must be a HeadsArgs")
+    rc = (_LIB or lib()).sptmm_heads_norm_rotate(C.addressof(args), stream.handle if type(stream) is Stream else stream)
+    if rc < 0:
+        _ck(rc)
 
 
 def attention_workspace_bytes(args: AttentionArgs) -> int:
@@ -590,7 +594,12 @@ def attention_workspace_bytes(args: AttentionArgs) -> int:
 
 def attention(args: AttentionArgs, workspace=None, workspace_bytes: int = 0, stream: "Stream | int | None" = None):
     """Causal attention with grouped heads over packed sequences against a cache of rows."""
-    _ck(lib().sptmm_attention(C.byref(args), _dev(workspace), workspace_bytes, _stream(stream)))
+    if type(args) is not AttentionArgs:
+        raise TypeError("args must be an AttentionArgs")
+    rc = (_LIB or lib()).sptmm_attention(C.addressof(args), workspace.ptr if type(workspace) is DeviceBuffer else workspace, workspace_bytes,
+                                         stream.handle if type(stream) is Stream else stream)
+    if rc < 0:
+        _ck(rc)
 
 
 class Adapters:
@@ -610,7 +619,9 @@ class Adapters:
 
     def apply(self, X, row_slot, M: int, base, Y, workspace, workspace_bytes: int, stream: "Stream | int | None" = None):
         """Y[m] = base[m] + scale * B (A X[m]) with the adapter in slot row_slot[m] (int32 on the device; outside: none); base may be Y or None."""
-        _ck(lib().sptmm_adapters_apply(self.handle, _dev(X), _dev(row_slot), M, _dev(base), _dev(Y), _dev(workspace), workspace_bytes, _stream(stream)))
+        rc = (_LIB or lib()).sptmm_adapters_apply(self.handle, _dev(X), _dev(row_slot), M, _dev(base), _dev(Y), _dev(workspace), workspace_bytes, _stream(stream))
+        if rc < 0:
+            _ck(rc)
 
     def free(self):
         if self.handle:

@@ -41,6 +41,10 @@ def test_attention_of_nothing_is_a_call_without_work():
     sp.attention(attention_args(total_q=0, q=None, out=None), None, 0)
     with pytest.raises(AttributeError):
         sp.AttentionArgs(head_size=64)
+    with pytest.raises(TypeError):
+        sp.attention(heads_args(), None, 0)
+    with pytest.raises(TypeError):
+        sp.heads_norm_rotate(attention_args())
 
 
 def heads_args(**changes):
