@@ -286,6 +286,7 @@ def run(argv=None):
                          "density (the headline shape at 3.7-25 % nonzeros against i2s), "
                          "plans (the launch-shape model against sptmm_weights_tune over random shapes), "
                          "q8 (the headline shape through the int8, scaled-int8 and quantising calls, one call at a time), "
+                         "block (not on by default: the attention half of the decoder layer, stage by stage and as a HIP graph), "
                          "copy (4 launches of a 1 GiB copy kernel, for counter calibration), ceiling (a pure streaming "
                          "read of as many bytes as one step moves); profiling runs use --legs none or one leg")
     ap.add_argument("--detail", default=os.path.join(ROOT, "gpurun_out", "bench_detail.json"),
@@ -539,6 +540,8 @@ def run(argv=None):
     plans = plans_leg(sp) if "plans" in legs else None
     quantising = quantising_leg(sp, st, K, N, S, calls=min(a.reps or 600, 600)) if "q8" in legs else None
 
+    block = block_leg(sp, st, calls=min(a.reps or 200, 200)) if "block" in legs else None
+
     gbps = nbytes / us_gemv / 1e3
     traffic, traffic_src = None, None
     if os.path.exists(TRAFFIC_SIDECAR):
@@ -574,6 +577,7 @@ def run(argv=None):
         },
         "single_launch": single, "other_encodings": others, "configs": configs, "layer_sequence": layer_seq, "density_sweep": density, "launch_plans": plans,
         "quantising_calls": quantising,
+        **({"attention_block": block} if block else {}),
         "device": {"arch": info["arch"], "compute_units": info["compute_units"]},
         "roofline": {"bound": "hbm", "achieved": round(gbps, 1), "peak": PEAK_GBPS, "unit": "GB/s",
                      "frac": round(gbps / PEAK_GBPS, 4), "traffic": traffic, "traffic_source": traffic_src,
@@ -657,6 +661,86 @@ def final_line(full):
     return json.dumps(out, ensure_ascii=False, separators=(",", ":"))
 
 
+def block_leg(sp, st, calls=200):
+    """The attention half of the decoder layer of config 3 (20 query and 5 key/value heads of 128) as a program runs it, one
+    launch sequence per pass: q+k+v projection (quantised bf16 rows, u16 lists) -> adapters (8 slots of rank 16) -> norms,
+    rotation and cache rows -> attention -> o projection -> adapters; four requests decoding one token each against 2000
+    cached ones, and one prompt of 1024.  Microseconds per stage (host clock around `calls` launches and a stream
+    synchronise) and per pass, eager and as a HIP graph; the weights of one layer, warm."""
+    import numpy as np
+
+    K, HQ, HKV, D = 2560, 20, 5, 128
+    n_qkv, n_o = (HQ + 2 * HKV) * D, HQ * D
+    r = np.random.default_rng(1)
+
+    def bf16(*shape):
+        return (r.standard_normal(shape).astype(np.float32).view(np.uint32) >> 16).astype(np.uint16)
+
+    rows = []
+    for name, nq, nk in (("4 requests, one token each", [1] * 4, [2000] * 4), ("one prompt", [1024], [1024])):
+        T, B = sum(nq), len(nq)
+        ws = [sp.Weights.upload_u16(*sp.generate_ternary(K, n, 1536)[1:], K, 0, rows=min(T, 8)) for n in (n_qkv, n_o)]
+        sets = [sp.Adapters(K, n, sp.X_BF16, 8, 16) for n in (n_qkv, n_o)]
+        for a, n in zip(sets, (n_qkv, n_o)):
+            A, Bm = sp.DeviceBuffer.from_numpy(bf16(16, K)), sp.DeviceBuffer.from_numpy(bf16(n, 16))
+            for slot in range(8):
+                a.set(slot, A, Bm, 16, 0.01, st)
+            st.sync()
+            A.free(), Bm.free()
+        cap = max(nk) * B
+        buf = {k: sp.DeviceBuffer.from_numpy(v) for k, v in (
+            ("x", bf16(T, K)), ("slot", (np.repeat(np.arange(B), nq) % 8).astype(np.int32)), ("k", bf16(cap, HKV * D)), ("v", bf16(cap, HKV * D)), ("q", bf16(T, n_o)), ("att", bf16(T, n_o)),
+            ("y", np.zeros((T, n_qkv), np.float32)), ("z", np.zeros((T, n_o), np.float32)), ("gain", np.ones(D, np.float32)), ("len", np.array(nk, np.int32)),
+            ("first", np.concatenate([[0], np.cumsum(nq)]).astype(np.int32)), ("start", (np.arange(B) * max(nk)).astype(np.int32)),
+            ("pos", np.concatenate([np.arange(m - n, m) for n, m in zip(nq, nk)]).astype(np.int32)),
+            ("row", np.concatenate([b * max(nk) + np.arange(m - n, m) for b, (n, m) in enumerate(zip(nq, nk))]).astype(np.int32)))}
+        heads = sp.HeadsArgs(q=buf["y"], k=buf["y"].ptr.value + 4 * n_o, v=buf["y"].ptr.value + 4 * (n_o + HKV * D), q_stride=n_qkv, k_stride=n_qkv, v_stride=n_qkv, in_type=sp.X_F32,
+                             out_type=sp.X_BF16, q_out=buf["q"], k_out=buf["k"], v_out=buf["v"], q_out_stride=n_o, k_out_stride=HKV * D, v_out_stride=HKV * D, tokens=T, q_heads=HQ,
+                             kv_heads=HKV, head_dim=D, positions=buf["pos"], kv_rows=buf["row"], kv_capacity=cap, q_gain=buf["gain"], k_gain=buf["gain"], eps=1e-5,
+                             rotation=sp.Rotation([10000.0 ** (-2.0 * j / D) for j in range(D // 2)]))
+        attn = sp.AttentionArgs(q=buf["q"], k=buf["k"], v=buf["v"], out=buf["att"], q_stride=n_o, k_stride=HKV * D, v_stride=HKV * D, out_stride=n_o, kv_rows=cap, q_start=buf["first"],
+                                kv_start=buf["start"], kv_len=buf["len"], batch=B, total_q=T, max_q=max(nq), max_kv=max(nk), q_heads=HQ, kv_heads=HKV, head_dim=D, type=sp.X_BF16,
+                                scale=D ** -0.5)
+        need = max([16, sp.attention_workspace_bytes(attn)] + [a.workspace_bytes(T) for a in sets] + [w.q8_workspace_bytes(T) for w in ws])
+        work = sp.DeviceBuffer(need)
+
+        def project(i, x, y):
+            ws[i].gemv_q8_ws(x, 2, T, 0.02, y, work, need, st)
+
+        stages = (("qkv_projection", lambda: project(0, buf["x"], buf["y"])),
+                  ("qkv_adapters", lambda: sets[0].apply(buf["x"], buf["slot"], T, buf["y"], buf["y"], work, need, st)),
+                  ("heads", lambda: sp.heads_norm_rotate(heads, st)),
+                  ("attention", lambda: sp.attention(attn, work, need, st)),
+                  ("o_projection", lambda: project(1, buf["att"], buf["z"])),
+                  ("o_adapters", lambda: sets[1].apply(buf["att"], buf["slot"], T, buf["z"], buf["z"], work, need, st)))
+
+        def timed(f):
+            for _ in range(10):
+                f()
+            st.sync()
+            t0 = time.perf_counter()
+            for _ in range(calls):
+                f()
+            st.sync()
+            return round((time.perf_counter() - t0) / calls * 1e6, 2)
+
+        row = {"case": name, "tokens": T, "stages_us": {n: timed(f) for n, f in stages}}
+
+        def whole():
+            for _, f in stages:
+                f()
+
+        row["eager_us"] = timed(whole)
+        with sp.Graph(st) as g:
+            whole()
+        row["graph_us"] = timed(lambda: g.launch(st))
+        rows.append(row)
+        g.destroy()
+        for o in list(buf.values()) + ws + sets + [work]:
+            o.free()
+    return {"rows": rows, "protocol": "host clock around %d passes + stream synchronise; one layer's weights, warm" % calls}
+
+
 def main():
     full = run()
     path = full.get("detail_file")
@@ -668,7 +752,7 @@ def main():
                 json.dump(full, f, ensure_ascii=False, indent=1)
         except OSError as e:  # a read-only tree: the tables still go to stderr
             print("bench.py: cannot write %s: %s" % (path, e), file=sys.stderr)
-    for leg in ("single_launch", "other_encodings", "configs", "layer_sequence", "density_sweep", "launch_plans", "quantising_calls"):
+    for leg in ("single_launch", "other_encodings", "configs", "layer_sequence", "density_sweep", "launch_plans", "quantising_calls", "attention_block"):
         if full.get(leg):
             print(json.dumps({leg: full[leg]}, ensure_ascii=False), file=sys.stderr)
     print(final_line(full), flush=True)
