@@ -288,48 +288,61 @@ template <int T, int DP, int KT> struct Rows {
     {
         const int half = (threadIdx.x & 63) >> 5;
         f32x16 s[KB];
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[b][e] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
-                s[b] = mfma<T>(*reinterpret_cast<const u16x8 *>(k + (k_at ^ (ks << 5)) + b * 32 * DP * 2), qf[ks], s[b]);
-        if (KIND == EDGE && j0 + KT - 1 > lo) {
-            const int last = lim - j0 - 4 * half;
+        auto score = [&] {
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[b][e] = b * 32 + 8 * (e >> 2) + (e & 3) <= last ? s[b][e] : -INFINITY;
-        }
-        float mx = s[0][0];
+                for (int e = 0; e < 16; ++e) s[b][e] = 0.f;
 #pragma unroll
-        for (int b = 0; b < KB; ++b)
+            for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
-        mx = halves_max(mx);
-        if (__ballot((mx - top) * p.c > 8.f)) {
-            const float now = fmaxf(top, mx), f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - now) * p.c);
+                for (int b = 0; b < KB; ++b)
+                    s[b] = mfma<T>(*reinterpret_cast<const u16x8 *>(k + (k_at ^ (ks << 5)) + b * 32 * DP * 2), qf[ks], s[b]);
+            if (KIND == EDGE && j0 + KT - 1 > lo) {
+                const int last = lim - j0 - 4 * half;
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[b][e] = b * 32 + 8 * (e >> 2) + (e & 3) <= last ? s[b][e] : -INFINITY;
+            }
+        };
+        u16x8 pf[2 * KB];
+        // the weights relative to `top`, rounded into pf; their 32-bit sum.  fp16: p is held 2^7 larger, so that what rounds to zero is
+        // below 2^-32 of the largest.
+        auto weigh = [&] {
+            const float at = (top == -INFINITY ? 0.f : top * p.c) - (T == SPTMM_X_F16 ? 7.f : 0.f);
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[b][e], p.c, -at));
+                    part[e & 3] += x;
+                    pf[2 * b + (e >> 3)][e & 7] = narrow<T>(x);
+                }
+            return (part[0] + part[1]) + (part[2] + part[3]);
+        };
+        score();
+        float tile_sum = weigh();
+        // Weights relative to an old maximum are as good as any while they fit: only where they outgrow 2^15 (or there is no maximum
+        // yet) is the tile's maximum looked for and followed, and the tile weighed again.  An fp16 weight is then below 2^16 always.
+        if (__ballot(tile_sum > 32768.f || top == -INFINITY)) {
+            score();
+            float mx = s[0][0];
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
+            const float now = fmaxf(top, halves_max(mx)), f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - now) * p.c);
 #pragma unroll
             for (int d = 0; d < DS; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[d][e] *= f;
             sum *= f;
             top = now;
+            tile_sum = weigh();
         }
-        // fp16: p is held 2^7 larger, so that what rounds to zero is below 2^-32 of the largest (top may lag by 2^8: 2^15 at most)
-        const float at = (top == -INFINITY ? 0.f : top * p.c) - (T == SPTMM_X_F16 ? 7.f : 0.f);
-        u16x8 pf[2 * KB];
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[b][e], p.c, -at));
-                sum += x;
-                pf[2 * b + (e >> 3)][e & 7] = narrow<T>(x);
-            }
+        sum += tile_sum;
         if (KIND == EDGE && bad) {
             const f32x16 zero = {0.f};
 #pragma unroll
@@ -440,6 +453,7 @@ template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64
         load(i + 1, k_a, v_a);
         if (j <= hi) r.template step<R::EDGE>(p, k_b, v_b, j, lo, r.polluted(v_b, j, end, lo));
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing is on its way into the LDS when the workgroup gives it up)
     const float sum = halves_sum(r.sum), f = p.splits > 1 ? 1.f : 1.f / sum;
     if (!valid) return;
     const bool none = r.lim < 0;
