@@ -558,6 +558,8 @@ extern "C" int sptmm_adapters_apply(const sptmm_adapters *a, const uint16_t *X, 
     const size_t want = need(a, M);
     if (want && (!workspace || workspace_bytes < want))
         return fail(SPTMM_ERR_INVALID, "the workspace has %zu bytes, %zu are needed", workspace ? workspace_bytes : (size_t)0, want);
+    // (a dimension of a launch holds 2^32 work-items)
+    if ((int64_t)((M + 15) / 16) * ((a->n_pairs + 3) / 4) >= (1 << 24)) return fail(SPTMM_ERR_UNSUPPORTED, "M = %d rows by N = %d columns are more than one launch holds", M, a->N);
     if (int rc = check_device(a)) return rc;
     AdapterArgs p{};
     p.X = X, p.A = a->A, p.B = a->B, p.row_slot = row_slot, p.info = a->info, p.base = base, p.h = (float *)workspace, p.Y = Y;

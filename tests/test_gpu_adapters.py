@@ -115,6 +115,12 @@ def test_many_rows(t):
     s.free()
 
 
+def test_many_rows_of_the_largest_rank():
+    s = Set(12, 32, 2064, "bf16", [256, 3, 250], 256)
+    s.check(1, np.arange(2100) // 30 % 4 - 1)
+    s.free()
+
+
 @pytest.mark.parametrize("rank,max_rank", [(1, 256), (64, 64), (65, 128), (200, 256), (256, 256)])
 def test_large_ranks(rank, max_rank):
     s = Set(3, 320, 96, "bf16", [rank, 5], max_rank)
@@ -219,6 +225,9 @@ def test_refusals():
               (X, S, 3, None, Y, ws, n - 1), (X, S, (1 << 24) + 1, None, Y, ws, n), (off, S, 3, None, Y, ws, n), (X, S.ptr.value + 2, 3, None, Y, ws, n), (X, S, 3, Y.ptr.value + 4, Y, ws, n)):
         with pytest.raises(sp.SptmmError):
             s.a.apply(*a)
+    with pytest.raises(sp.SptmmError) as e:  # more tiles than a launch has work-items
+        Set(1, 16, 1 << 14, "f16", [1]).a.apply(X, S, 1 << 24, None, Y, ws, 1 << 60)
+    assert e.value.code == -2
     for a in ((-1, X, Y, 4, 1.0), (2, X, Y, 4, 1.0), (0, X, Y, 65, 1.0), (0, X, Y, -1, 1.0), (0, None, Y, 4, 1.0), (0, X, None, 4, 1.0), (0, X, Y, 4, float("nan")), (0, X, Y, 4, float("inf"))):
         with pytest.raises(sp.SptmmError):
             s.a.set(*a)
