@@ -334,8 +334,9 @@ int sptmm_gemv_batched(const sptmm_weights *const *ws, const void *const *X_dev,
  *     Y[m][n] = base[m][n] + scale_s * sum_r B_s[n][r] * (sum_k A_s[r][k] X[m][k]),   s = row_slot[m]
  * A set holds `slots` adapters for one K x N projection, each of any rank up to max_rank (1..256), weights fp16 or bf16
  * (sptmm_xtype).  Products of 16-bit values are summed in 32 bits, and the inner sums stay in 32 bits.
- *   sptmm_adapters_set: copies A [rank][K] and B [N][rank] (dense row-major device buffers) into a slot, on `stream`; rank 0 empties it.
- *     The caller orders it against sptmm_adapters_apply calls that use the slot on other streams.
+ *   sptmm_adapters_set: copies A [rank][K] and B [N][rank] (dense row-major device buffers, which stay as they are until `stream`
+ *     has passed the copy) into a slot, on `stream`; rank 0 empties it.  The caller orders it against sptmm_adapters_apply calls
+ *     that use the slot on other streams.
  *   sptmm_adapters_apply: X [M][K] of the set's type (what sptmm_gemv_q8 takes), base and Y [M][N] float (what it leaves).
  *     base may be Y (added in place) or NULL (zeros).  row_slot[m] outside 0..slots-1, or an empty slot: Y[m] = base[m].
  *     Rows of one slot need not lie together.  An Inf or NaN in one row or one adapter reaches the rows that use it only.
@@ -386,8 +387,8 @@ int sptmm_heads_norm_rotate(const sptmm_heads_args *args, void *stream);
 /* Causal attention with grouped heads over packed sequences.  Sequence b has the query rows q_start[b] .. q_start[b+1]-1 of q
  * and the keys and values kv_start[b] .. kv_start[b]+kv_len[b]-1 of the cache; its query i of n sees keys j <= kv_len[b] - n + i
  * (whole prompts: n = kv_len; one token against a cache: n = 1; chunks of prompts in between; rows that see nothing become
- * zeros).  kv_start and kv_len NULL: the keys are packed as the queries are.  Query head h reads key/value head
- * h / (q_heads / kv_heads).  16-bit inputs and outputs; products summed, and softmax statistics kept, in 32 bits.
+ * zeros).  kv_start and kv_len NULL: the keys are packed as the queries are (k and v have at
+ * least q_start[batch] rows).  Query head h reads key/value head h / (q_heads / kv_heads).  `out` overlaps no input.  16-bit inputs and outputs; products summed, and softmax statistics kept, in 32 bits.
  * Output row i depends on the keys and values it sees only: Inf or NaN in other rows of the cache do not reach it.  Rows of
  * `out` behind the last sequence are left as they were.
  * max_q and max_kv (host side: at least the longest sequence's queries and keys) choose how the work is cut up; the results
@@ -401,10 +402,10 @@ typedef struct sptmm_attention_args {
     int64_t kv_rows;                                  /* rows of k and v, at most 2^30 */
     const int32_t *q_start;                           /* [batch + 1], not decreasing, q_start[batch] <= total_q */
     const int32_t *kv_start, *kv_len;                 /* [batch] each, or both NULL */
-    int batch, total_q, max_q, max_kv;
-    int q_heads, kv_heads, head_dim;                  /* head_dim a multiple of 8, 8..256 */
+    int batch, total_q, max_q, max_kv;                /* batch * kv_heads at most 2^22, total_q * q_heads at most 2^29 */
+    int q_heads, kv_heads, head_dim;                  /* q_heads a multiple of kv_heads, at most 65535; head_dim a multiple of 8, 8..256 */
     int type;                                         /* SPTMM_X_F16 or SPTMM_X_BF16 */
-    float scale;                                      /* of the scores, positive */
+    float scale;                                      /* of the scores, positive, below 1e30 */
 } sptmm_attention_args;
 size_t sptmm_attention_workspace_bytes(const sptmm_attention_args *args);
 int sptmm_attention(const sptmm_attention_args *args, void *workspace_dev, size_t workspace_bytes, void *stream);
@@ -432,7 +433,7 @@ int sptmm_event_elapsed_us(void *start, void *stop, double *us);
  * (join) -- independent projections then sit on parallel branches of the graph. */
 int sptmm_stream_wait_event(void *stream, void *event);
 /* Stream capture: the launches issued on `stream` between _begin and _end (any of
- * the sptmm_gemv_* calls, in any mix) become one executable HIP graph that
+ * the sptmm_gemv_* calls, sptmm_adapters_set / _apply, sptmm_heads_norm_rotate and sptmm_attention, in any mix) become one executable HIP graph that
  * _launch replays -- a decoder layer's fixed sequence of projections as one
  * submission.  The reference issues its kernels one by one with a device
  * synchronize after each (main.cu:767-782).  Pointers and shapes are frozen at

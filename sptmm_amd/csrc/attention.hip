@@ -17,9 +17,8 @@
 // their order.
 //
 // Rounding: products of 16-bit values summed in 32 bits; statistics, sums and rescaling in 32 bits; p is rounded to 16 bits
-// for the second product (bf16: half a step is 2^-9 of p at most 1, and the terms' errors average out), the result once.
-// A running maximum is followed only when it is passed by more than 2^8 (the sums then hold values up to 2^8 relative to it,
-// far from the ends of every type used): most tiles rescale nothing.
+// for the second product (half a step of p each, bf16 2^-8 and fp16 2^-11 of it: the terms' errors average out), the result once.
+// The maximum is followed only where weights relative to the last one outgrow 2^15: most tiles look for none and rescale nothing.
 #include <cmath>
 
 #include "internal.hpp"
@@ -48,7 +47,7 @@ struct AttnParams {
     int slots;      // row tiles, over all sequences (an upper bound)
     int splits, chunk;
     float *part_o;  // [split][query * q_heads + head][dim], unnormalised
-    float2 *part_ml;  // [split][query * q_heads + head]: maximum (of raw scores), sum
+    float2 *part_ml;  // [split][query * q_heads + head]: the maximum that the sums are relative to (of raw scores), sum
 };
 
 template <int T> __device__ __forceinline__ f32x16 mfma(u16x8 a, u16x8 b, f32x16 c)
@@ -130,50 +129,6 @@ template <int LOG_TM> __device__ __forceinline__ bool find_tile(const AttnParams
     t->rows = t->nq * p.group;
     t->row0 <<= LOG_TM;
     return t->row0 >= 0 && t->row0 < t->rows;
-}
-
-// The same in the order of the tiles' last keys, the furthest first, over all sequences: a tile's work is proportional to the keys it
-// sees, and workgroups that are dispatched late should be short.  Tile t of a sequence is placed at v = t + (keys before its
-// queries, in tiles); sequence b covers the places off .. off + tiles - 1.  With a sequence in every lane, the place of tile
-// `rank` is found by evaluating, at 64 places at a time, how many tiles lie at or behind the place.
-constexpr int BY_WORK = 32;  // sequences, at most (the evaluation walks them)
-template <int LOG_TM> __device__ __forceinline__ bool find_tile_by_work(const AttnParams &p, int rank, Tile *t)
-{
-    const int lane = threadIdx.x & 63;
-    const Seq s = sequence(p, min(lane, p.batch - 1));
-    const int tiles = lane < p.batch ? (int)(((int64_t)s.nq * p.group + (1 << LOG_TM) - 1) >> LOG_TM) : 0;
-    const int off = (int)(((int64_t)(s.nk - s.nq) * p.group) >> LOG_TM), behind = off + tiles;
-    int lo = 0x7fffffff, hi = -0x7fffffff;
-    for (int i = 0; i < p.batch; ++i)
-        if (__builtin_amdgcn_readlane(tiles, i) > 0) {
-            lo = min(lo, __builtin_amdgcn_readlane(off, i));
-            hi = max(hi, __builtin_amdgcn_readlane(behind, i));
-        }
-    if (lo >= hi) return false;
-    int64_t count;
-    int at;
-    for (int64_t stride = ((int64_t)hi - lo + 63) / 64;; stride = (stride + 63) / 64) {
-        const int64_t v = lo + lane * stride;
-        count = 0;
-        for (int i = 0; i < p.batch; ++i)
-            count += min(max((int64_t)__builtin_amdgcn_readlane(behind, i) - v, (int64_t)0), (int64_t)__builtin_amdgcn_readlane(tiles, i));
-        const int c = __popcll(__ballot(count > rank));
-        if (c == 0) return false;  // (there are no more than `rank` tiles)
-        at = c - 1;
-        if (stride == 1) break;
-        lo += (int)(at * stride);
-    }
-    const int place = lo + at, have = (int)__shfl((long long)count, at, 64);
-    unsigned long long who = __ballot(lane < p.batch && off <= place && place < behind);
-    for (int r = rank - (have - __popcll(who)); r > 0; --r) who &= who - 1;
-    const int seq = __builtin_amdgcn_readfirstlane(__builtin_ctzll(who));
-    t->q0 = __builtin_amdgcn_readlane(s.q0, seq);
-    t->nq = __builtin_amdgcn_readlane(s.nq, seq);
-    t->k0 = __builtin_amdgcn_readlane(s.k0, seq);
-    t->nk = __builtin_amdgcn_readlane(s.nk, seq);
-    t->rows = t->nq * p.group;
-    t->row0 = (place - __builtin_amdgcn_readlane(off, seq)) << LOG_TM;
-    return true;
 }
 
 // ------------------------------------------------------------------------------------------------ tiles in the LDS
@@ -391,6 +346,10 @@ template <int T> __device__ __forceinline__ void write4(const AttnParams &p, con
 }
 
 // ------------------------------------------------------------------------------------------------ TILE: rows over wavefronts
+// Bound by the matrix units' feed: one prompt of 8192 tokens, 20 heads of 128 on 5, bf16: 344 GFLOP in 325 to 345 us, 1.0 to 1.06 PFLOP/s, where a
+// product of two 8192 x 8192 matrices reaches 1.21 on the same card.  64 KB of LDS leave two workgroups to a compute unit, and
+// one's exponentials run beside the other's products; of the time, the exponentials alone are a tenth, the loads 3 %.  Four
+// wavefronts of 32 rows share each tile of K and V through the LDS (without bank conflicts); of 256 rows: slower, one workgroup a unit.
 template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) attention_tile_kernel(const AttnParams p)
 {
     static_assert(WAVES == 4, "128 rows");
@@ -398,15 +357,11 @@ template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64
     __shared__ __attribute__((aligned(1024))) char k_a[KT * DP * 2], k_b[KT * DP * 2], v_a[KT * DP * 2], v_b[KT * DP * 2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Tile t;
-    // The rows that see the most keys first, and of all heads before the next rows: workgroups dispatched late are short.
-    // Workgroups go to the eight XCDs in turn, and those that read the same head's keys should share an L2: without splits the
-    // tiles are dealt into eight hands, and each XCD takes as many neighbouring hands as there are heads, of at most two or
-    // three heads then (one prompt of 8192 tokens, 5 heads: a fifth of the reads that miss L2).  With splits the heads' parts
-    // differ in work by split, and are spread as they come.
-    const unsigned heads = (unsigned)p.kv_heads;
-    const unsigned x = blockIdx.x, hand = x % 8 * heads + x / 8 % heads;
-    const int kv_head = (int)(p.splits > 1 ? x % heads : hand / 8), split = blockIdx.z, rank = (int)(p.splits > 1 ? x / heads : x / 8 / heads * 8 + hand % 8);
-    if (p.batch <= BY_WORK ? !find_tile_by_work<LOG_TM>(p, rank, &t) : !find_tile<LOG_TM>(p, p.slots - 1 - rank, &t)) return;
+    // A sequence's last rows, which see the most keys, first, and of all heads before the next rows: workgroups dispatched late
+    // are short.  (All sequences' tiles in one order of the keys they see: eight chunks of up to 400 tokens 361 us, so 371; thirty
+    // prompts of 30 to 1500 tokens 170, so 150.  Heads kept to their XCDs' L2s: one prompt of 8192, 5 heads, 341 and 346; 32 heads 524 and 510.)
+    const int kv_head = (int)(blockIdx.x % (unsigned)p.kv_heads), split = blockIdx.z, slot = p.slots - 1 - (int)(blockIdx.x / (unsigned)p.kv_heads);
+    if (!find_tile<LOG_TM>(p, slot, &t)) return;
     const int i_last = (min(t.row0 + TM, t.rows) - 1) / p.group, all = min(t.nk, t.nk - t.nq + i_last + 1);
     const int begin = split * p.chunk, end = split == p.splits - 1 ? all : min(all, begin + p.chunk);
     if (split && begin >= end) return;
@@ -474,6 +429,9 @@ template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64
 }
 
 // ------------------------------------------------------------------------------------------------ KEYS: keys over wavefronts
+// Bound by the cache's read: 32 sequences of 2000 to 8000 keys, 661 MB, 5.5 TB/s.  Nothing is shared between wavefronts but the
+// sums at the end, so that each waits for its own loads only.  Two to a workgroup, as 128 KB of LDS for four leave one workgroup
+// to a compute unit: 20 heads of 128 on 5, one token against 8000 keys 13.7 us and 18.6, 32 against 1500 36 and 40, 64: 55 and 54.
 template <int T, int DP, int WAVES, bool STREAM> __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) attention_keys_kernel(const AttnParams p)
 {
     constexpr int KT = 32, LOG_TM = 5, ONE = KT * DP * 2;
@@ -577,8 +535,8 @@ template <int T, int DP, int WAVES, bool STREAM> __global__ void __launch_bounds
 
 // ------------------------------------------------------------------------------------------------ splits joined
 // Per (query, head) the splits that hold keys the row sees, added in a fixed order, by WAVES wavefronts: the four of a workgroup
-// where there are many splits (one row of 63: 13 us by a single wavefront, 4 by four), one where there are few and many
-// rows (870 x 20 rows of four: 33 us by four wavefronts each, 18 by one).
+// where there are many splits (one token of 20 heads against 8000 keys, 63 splits: the call 13.6 us, by single wavefronts
+// 16.8), one where there are few and many rows (870 x 20 rows of four: 204 us, by four wavefronts each 217).
 template <int T, int WAVES> __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
 {
     __shared__ __attribute__((aligned(16))) f32x4 parts[4][64];
@@ -663,9 +621,9 @@ int check(const sptmm_attention_args *a)
     if (a->q_heads < 1 || a->kv_heads < 1 || a->q_heads % a->kv_heads || a->q_heads > 65535)
         return fail(SPTMM_ERR_INVALID, "q_heads must be a positive multiple of kv_heads, at most 65535");
     if (a->head_dim < 8 || a->head_dim > 256 || a->head_dim % 8) return fail(SPTMM_ERR_INVALID, "head_dim must be a multiple of 8, 8..256");
-    if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail(SPTMM_ERR_INVALID, "scale must be positive and finite");
-    if ((int64_t)a->total_q * a->q_heads > 0x7fffffff - 256 || (int64_t)a->batch * a->kv_heads > (1 << 22))
-        return fail(SPTMM_ERR_INVALID, "total_q * q_heads must stay below 2^31, batch * kv_heads at most 2^22");
+    if (!(a->scale > 0.f) || !(a->scale < 1e30f)) return fail(SPTMM_ERR_INVALID, "scale must be positive and below 1e30");
+    if ((int64_t)a->total_q * a->q_heads > (1 << 29) || (int64_t)a->batch * a->kv_heads > (1 << 22))  // (2^32 work-items to a launch)
+        return fail(SPTMM_ERR_INVALID, "total_q * q_heads must be at most 2^29, batch * kv_heads at most 2^22");
     if (a->kv_rows > (1 << 30)) return fail(SPTMM_ERR_INVALID, "kv_rows must be at most 2^30");
     return SPTMM_OK;
 }
@@ -687,17 +645,23 @@ Cut cut(const sptmm_attention_args *a)
     const int64_t rows = (int64_t)a->total_q * group;
     c.slots = (int)(rows / tm + a->batch);
     // Workgroups without splits (those that have rows): about as many as sequences have tiles.  Splits where they are fewer than
-    // the chip holds -- of the KEYS form at least four per compute unit, of the TILE form two (one for heads of 256) --, yet
-    // three quarters of that in the TILE form: an exact fit leaves some units a third workgroup to do after the others (512 rows against 16000
-    // keys, 8 heads: 384 workgroups 109 us, 512 workgroups 132; four chunks of 130 to 250 tokens against 12000 to 20000: 201 and 190).
+    // the chip has places for -- two per compute unit, of the TILE form with heads of 256 one --, in the TILE form three quarters
+    // of that: 512 tokens against 16000 keys, 8 heads: 113 us, with all the places 134; eight chunks of 64 tokens against 3000
+    // to 9000, 5 heads: 67 and 75; four chunks of 130 to 250 against 12000 to 20000, 5 heads: 214 and 200.
     const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>(c.slots, c.keys ? (int64_t)a->batch : rows / tm + 1)) * a->kv_heads;
     const int64_t room = c.keys ? 512 : c.dp == 256 ? 192 : 384;
     const int max_kv = (int)std::min<int64_t>(a->max_kv, a->kv_rows);
-    const int unit = c.keys ? 128 : 512;  // keys a workgroup should have at least
+    // Keys a workgroup should have at least.  Where the queries are most of the keys, half the tiles see little of a late split
+    // and the join has many rows: one prompt of 600, 1024, 1500 tokens, 20 heads on 5: 19, 25, 35 us at 2048, 27, 32, 48 at 512
+    // (2000 tokens, 8 heads on 2: 40 and 36).  A chunk of 64 against 1500, of 200 against 2000: 32, 41 us at 2048, 21, 25 at 512.
+    const int unit = c.keys ? 128 : 2ll * a->max_q >= max_kv ? 2048 : 512;
     const int64_t want = (room + tiles - 1) / tiles, most = (max_kv + unit - 1) / unit;
     c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
+    if ((int64_t)a->total_q * a->q_heads >= (1 << 24)) c.splits = 1;  // (one launch of the join holds fewer rows)
     c.chunk = std::max(unit, (max_kv / c.splits + 127) / 128 * 128);
     c.splits = std::max(1, std::min(c.splits, (max_kv + c.chunk - 1) / c.chunk));
+    // Caches that no level below holds between two calls are read past them: 661 MB 120 us (5.5 TB/s), through them 133; 246 MB 55
+    // and 61.  Below, no way wins: 123 MB 33.8 and 35.9, 33 MB 14.3 and 13.6.
     c.stream = (int64_t)a->batch * max_kv * a->kv_heads * a->head_dim * 4 > (128ll << 20);
     return c;
 }
@@ -711,7 +675,7 @@ size_t workspace(const sptmm_attention_args *a, const Cut &c)
 
 template <int T> void launch(const AttnParams &p, const Cut &c, hipStream_t st)
 {
-    const dim3 grid = c.keys ? dim3(c.slots, p.kv_heads, c.splits) : dim3((unsigned)(c.splits > 1 ? c.slots : (c.slots + 7) / 8 * 8) * p.kv_heads, 1, c.splits);
+    const dim3 grid = c.keys ? dim3(c.slots, p.kv_heads, c.splits) : dim3((unsigned)c.slots * p.kv_heads, 1, c.splits);
     if (c.keys) {
         const auto kernel = c.dp == 64    ? (c.stream ? attention_keys_kernel<T, 64, 2, true> : attention_keys_kernel<T, 64, 2, false>)
                             : c.dp == 128 ? (c.stream ? attention_keys_kernel<T, 128, 2, true> : attention_keys_kernel<T, 128, 2, false>)

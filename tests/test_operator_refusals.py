@@ -17,9 +17,9 @@ def attention_args(**changes):
 @pytest.mark.parametrize("changes", [
     dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(q_start=None), dict(kv_start=None), dict(kv_len=None), dict(type=0), dict(type=sp.X_F32), dict(batch=-1), dict(total_q=-1),
     dict(max_q=-1), dict(max_kv=-1), dict(kv_rows=-1), dict(kv_rows=(1 << 30) + 1), dict(q_heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(q_heads=65536, kv_heads=1), dict(head_dim=0),
-    dict(head_dim=4), dict(head_dim=60), dict(head_dim=264), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(q_stride=255), dict(q_stride=248),
+    dict(head_dim=4), dict(head_dim=60), dict(head_dim=264), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(scale=1e30), dict(q_stride=255), dict(q_stride=248),
     dict(k_stride=120), dict(v_stride=132), dict(out_stride=252), dict(out_stride=258), dict(k_stride=(1 << 22) + 8), dict(q=4098), dict(k=8200), dict(v=12290), dict(out=16388),
-    dict(q_start=66), dict(kv_start=65), dict(kv_len=67), dict(total_q=1 << 29, q_heads=4), dict(batch=1 << 25)])
+    dict(q_start=66), dict(kv_start=65), dict(kv_len=67), dict(total_q=1 << 29, q_heads=4), dict(total_q=(1 << 27) + 1, q_heads=4), dict(batch=1 << 25)])
 def test_attention_refuses(changes):
     with pytest.raises(sp.SptmmError) as e:
         sp.attention(attention_args(**changes), 4096, 1 << 40)
@@ -34,6 +34,8 @@ def test_attention_wants_its_workspace():
         with pytest.raises(sp.SptmmError):
             sp.attention(a, ws, size)
     assert sp.attention_workspace_bytes(attention_args(head_dim=60)) == 0
+    # few sequences in very many rows: not split, as one launch of the join holds less than 2^24 rows
+    assert sp.attention_workspace_bytes(attention_args(batch=1, total_q=1 << 22, max_q=1, max_kv=10000, kv_rows=10000)) == 0
 
 
 def test_attention_of_nothing_is_a_call_without_work():
