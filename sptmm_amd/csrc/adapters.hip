@@ -2,7 +2,7 @@
 //
 //   Y[m][n] = base[m][n] + scale_s * sum_r B_s[n][r] * h[m][r],   h[m][r] = sum_k A_s[r][k] X[m][k],   s = row_slot[m]
 //
-// Two launches.  The first makes h: 16 rows of X against 16 ranks of A per matrix instruction (16-bit operands, 32-bit
+// In general two launches.  The first makes h: 16 rows of X against 16 ranks of A per matrix instruction (16-bit operands, 32-bit
 // sums), the rows' contraction over K split over wavefronts and workgroups.  The second adds up the splits' partial sums in
 // their order and multiplies by B on the 32-bit matrix instruction: h is never rounded to 16 bits -- outputs are 32-bit
 // floats, and a rounded h would cost them fifteen of their bits -- and B's 16-bit values are exact in 32.
@@ -12,6 +12,10 @@
 // and never by a product with zero: an infinity in one adapter's weights reaches its own rows only.
 //
 // Both weights sit in the order in which a wavefront reads them, 1 KiB per load instruction (adapters_pack_kernel).
+//
+// Many rows are bound by base, Y and X: 3001 rows, K=2560 N=13824, eight slots of rank 16 to 64: 356 MB in 101 us, 3.5 TB/s (an
+// addition to an array of that size, 332 MB, 57 us).  A few rows are bound by latency: one row 6.7 to 8.3 us where an empty launch
+// takes 3.5; 48 rows of 32 slots, K=6912 N=2560: 18 MB in 13 to 15.5 us, two launches that each wait for slots, weights and sums.
 #include <atomic>
 #include <cmath>
 
@@ -436,14 +440,23 @@ template <int T> __global__ void __launch_bounds__(SHRINK_WAVES * 64) adapters_f
 
 int hip_fail(hipError_t e, const char *what) { return fail(SPTMM_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e); }
 
-// Up to this much of A (KiB of the largest slot), and one tile of rows, both products run in one launch.
-constexpr int FUSED_A_KIB = 160;
+// One tile of rows, and A small (KiB of the largest slot, and of all workgroups' reads if every row has another slot): both
+// products run in one launch.  K=2560 N=3840, one row: rank 32 (160 KiB) 8.1 us, in two launches 11.2; rank 64 (320) 8.3 and 10.8;
+// rank 128 (640) 13.4 and 11.1.  Sixteen rows of sixteen slots of rank 16: N=3840 (19 MiB) 8.1 and 10.7, N=13824 (68) 19.9 and 13.0;
+// eight rows (34) 10.7 both ways.
+constexpr int FUSED_A_KIB = 320, FUSED_READ_KIB = 32 << 10;
 
-bool fused(const sptmm_adapters *a, int M) { return M <= 16 && a->max_chunks * a->k_steps <= FUSED_A_KIB; }
+bool fused(const sptmm_adapters *a, int M)
+{
+    const int64_t kib = (int64_t)a->max_chunks * a->k_steps, groups = (a->n_pairs + SHRINK_WAVES - 1) / SHRINK_WAVES;
+    return M <= 16 && kib <= FUSED_A_KIB && kib * groups * M <= FUSED_READ_KIB;
+}
 
 // Workgroups that share the distinct slots of a tile.  Decode: every row may have another slot, and a workgroup that walks sixteen
 // waits for sixteen chains of loads; prompts: a tile rarely has more than two, and workgroups that find none cost their launch.
-int places_of(int M) { return M < 16 ? M : M <= 128 ? 16 : M <= 1024 ? 4 : 2; }
+// K=2560 N=3840, ranks 16 to 32, one, four or sixteen places: 64 rows of 64 slots 48, 22, 17 us; 256 rows of 64 slots 58, 36, 47;
+// 256 rows of prompts of 8 slots 13.5, 11.7, 14.0; 3001 rows, N=13824: 104, 101, 109.
+int places_of(int M) { return M < 16 ? M : M <= 128 ? 16 : 4; }
 
 // splits of K over workgroups: enough of them to fill the chip, each wavefront with two steps of 32 at least
 int splits_of(const sptmm_adapters *a, int M)
@@ -476,7 +489,10 @@ template <int T> void launch_apply(const AdapterArgs &p, bool one_launch, hipStr
     const int groups = (p.n_pairs + 3) / 4, z = p.places * ((p.max_chunks + CHUNKS_AT_ONCE - 1) / CHUNKS_AT_ONCE);
     const size_t lds = (size_t)p.max_chunks * 1024;
     hipLaunchKernelGGL((adapters_shrink_kernel<T>), dim3(p.tiles, p.splits, z), dim3(SHRINK_WAVES * 64), 0, st, p);
-    if ((int64_t)(p.tiles / 4) * groups < 512)  // (of the other kind there would be fewer than two workgroups per compute unit)
+    // Fewer workgroups of the many-row kind than this leave compute units idle.  K=2560, ranks 8 to 64 of 32 slots, rows in any order
+    // (in prompts), without and with it: 512 x 3840 (240 workgroups) 63, 65 us (16.8, 20.6); 1024 x 2560 (320) 78, 81 (18.9, 21.8);
+    // 512 x 6912 (432) 85, 72 (21.8, 22.7); 1024 x 6912 (864) 140, 105 (30.5, 26.6); 3001 x 13824 in prompts 127, 102.
+    if ((int64_t)(p.tiles / 4) * groups < 400)
         hipLaunchKernelGGL((adapters_expand_kernel<T, 1, false>), dim3(p.tiles * groups, 1, p.places), dim3(256), lds, st, p);
     else
         hipLaunchKernelGGL((adapters_expand_kernel<T, 4, true>), dim3((p.tiles + 3) / 4 * groups), dim3(256), 4 * lds, st, p);

@@ -9,7 +9,8 @@
 // to read, and no loss at far positions, where a product in 32 bits is off by position * 2^-24 radians.
 // Everything is computed in 32 bits and rounded once, to nearest even, on the way out.
 //
-// The pass is bound by its bytes.  A lane holds four pairs (eight elements: two loads of 16 bytes from float rows), so a
+// The pass is bound by its bytes: 4096 tokens, 20 + 5 + 5 heads of 128, float in, bf16 out, 94 MB in 18.8 us (5.0 TB/s);
+// 20011 tokens, 32 + 8 + 8 heads of 64, fp16, 246 MB in 50 us (4.9 TB/s); a large copy reaches 5.1.  A lane holds four pairs (eight elements: two loads of 16 bytes from float rows), so a
 // head of 128 takes 16 lanes and a wavefront handles four heads at a time; the sines of a token's four pairs stay in the
 // lane's registers while it walks the token's heads.
 #include <cmath>
@@ -146,7 +147,9 @@ __device__ __forceinline__ void turn(int position, unsigned turns_hi, unsigned t
     cosine = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, b) ^ ((quarter + 1) & 2) << 30);
 }
 
-constexpr int ROUNDS = 2;  // rounds of heads whose loads a wavefront has in flight together (four take registers that more wavefronts use better)
+// Rounds of heads whose loads a wavefront has in flight together.  4096 tokens, 20 + 5 + 5 heads of 128, float in: two 18.8 us, one
+// or four 19.7; 20011 tokens, 32 + 8 + 8 heads of 64, fp16 in: two 50, one 53, four 56 (registers that more wavefronts use better).
+constexpr int ROUNDS = 2;
 
 // IN: type of the rows; OUT: type of the heads written; INTER: pairs of neighbours (2j, 2j+1), else of halves (j, j + pairs);
 // WIDE: every run of four elements lies aligned for one load or store
@@ -321,7 +324,9 @@ extern "C" int sptmm_heads_norm_rotate(const sptmm_heads_args *a, void *stream)
     while ((8 << p.log_lanes) < a->head_dim) ++p.log_lanes;
     const int per_wave = 64 >> p.log_lanes, rounds = (p.heads + per_wave - 1) / per_wave;
     // One wavefront per round of heads while that leaves the chip's wavefront slots unfilled (a lone token: one round of
-    // latency instead of eight); one per token once there are enough tokens (its sines are computed once).
+    // latency instead of eight); one per token once there are enough tokens (its sines are computed once).  20 + 5 + 5 heads of
+    // 128, a wavefront per round and one per token: 64 tokens 7.4 us and 8.4, 512 7.7 and 9.2, 1024 9.4 and 10.0, 1500 11.6 and 11.0,
+    // 4096 27 and 19.
     p.parts = a->tokens >= 1024 ? 1 : rounds;
     const int rounds_per_part = (rounds + p.parts - 1) / p.parts;
     p.per_part = rounds_per_part * per_wave;

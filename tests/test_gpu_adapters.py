@@ -115,6 +115,21 @@ def test_many_rows(t):
     s.free()
 
 
+@pytest.mark.parametrize("M,K,N,rank", [(4, 2560, 384, 64), (1, 2560, 13824, 64), (2, 2592, 256, 64), (16, 2560, 13824, 16), (5, 2560, 13824, 16), (12, 6912, 2560, 16)])
+def test_sides_of_the_single_launch(M, K, N, rank):
+    """320 KiB of A a slot and more, and reads of A by all workgroups of 32 MiB and more."""
+    s = Set(13, K, N, "f16", [rank] * 17, rank)
+    s.check(1, np.arange(M) % 17)
+    s.free()
+
+
+@pytest.mark.parametrize("M", [512, 516, 390])
+def test_sides_of_the_many_row_form(M):
+    s = Set(14, 64, 6912, "bf16", [8, 0, 40, 64, 17], 64)  # 54 workgroups of columns to every 64 rows
+    s.check(1, np.arange(M) * 7 % 6 - 1)
+    s.free()
+
+
 def test_many_rows_of_the_largest_rank():
     s = Set(12, 32, 2064, "bf16", [256, 3, 250], 256)
     s.check(1, np.arange(2100) // 30 % 4 - 1)
