@@ -11,10 +11,10 @@
 // lie as the second product O^T = V^T P^T wants them -- its contraction over keys may run in any order, and V's rows are
 // read (transposed, from the LDS) in the order in which the lanes hold P.  P never leaves the registers.
 //
-// Two forms.  TILE (prompts): the wavefronts of a workgroup take 32 rows each and share tiles of 64 keys.  KEYS (single
-// tokens: all rows of a tile fit one wavefront's 32): every wavefront takes its own tiles of 32 keys.  Either may split the
-// keys over workgroups; unnormalised sums and statistics then go to a workspace and attention_join_kernel adds them up in
-// their order.
+// Two forms.  KEYS (single tokens: all rows of a tile fit one wavefront's 32): every wavefront takes its own tiles of 32 keys, and the
+// keys may be split over workgroups.  TILE (prompts): the wavefronts of a workgroup take 32 rows each and share tiles of 64 keys;
+// one workgroup per tile of 128 rows, or (few rows against many keys) workgroups with equal shares of all tiles' keys.
+// Unnormalised sums and statistics of parts go to a workspace, and attention_join_kernel adds them up in their order.
 //
 // Rounding: products of 16-bit values summed in 32 bits; statistics, sums and rescaling in 32 bits; p is rounded to 16 bits
 // for the second product (half a step of p each, bf16 2^-8 and fp16 2^-11 of it: the terms' errors average out), the result once.
@@ -45,9 +45,11 @@ struct AttnParams {
     int batch, total_q, q_heads, kv_heads, group, dim;
     float c;        // scale * log2(e)
     int slots;      // row tiles, over all sequences (an upper bound)
-    int splits, chunk;
-    float *part_o;  // [split][query * q_heads + head][dim], unnormalised
-    float2 *part_ml;  // [split][query * q_heads + head]: the maximum that the sums are relative to (of raw scores), sum
+    int splits, chunk;  // KEYS: of every sequence's keys
+    int log_rows;       // of a tile of the shares
+    int shares;         // TILE: workgroups that take equal shares of all tiles' blocks of keys; 0: one workgroup per tile
+    float *part_o;    // unnormalised sums: KEYS [split][query * q_heads + head][dim], TILE [share][0, 1][row of the tile][dim]
+    float2 *part_ml;  // likewise: the maximum that the sums are relative to (of raw scores), sum
 };
 
 template <int T> __device__ __forceinline__ f32x16 mfma(u16x8 a, u16x8 b, f32x16 c)
@@ -131,6 +133,98 @@ template <int LOG_TM> __device__ __forceinline__ bool find_tile(const AttnParams
     return t->row0 >= 0 && t->row0 < t->rows;
 }
 
+// Tiles of 128 rows and their keys as one row of blocks of 128 keys, for the sharing of the work: sequence by sequence, in it head by
+// head, tile by tile, all of a sequence's tiles with the blocks of all its keys (one at least, so that a tile without keys is
+// written too).  Found, like the tiles, by every wavefront from the sequences' arrays alone.
+constexpr int LOG_TILE = 7, TILE_ROWS = 1 << LOG_TILE, LOG_BLOCK = 7, LEAST_BLOCKS = 2 /* of a share */, MOST_SHARES = 512;
+
+__device__ __forceinline__ int tiles_of(const AttnParams &p, const Seq &s) { return (s.nq * p.group + (1 << p.log_rows) - 1) >> p.log_rows; }
+__device__ __forceinline__ int blocks_of(const Seq &s) { return max(1, (s.nk + (1 << LOG_BLOCK) - 1) >> LOG_BLOCK); }
+// of sequence b (none: 0)
+__device__ __forceinline__ int64_t seq_blocks(const AttnParams &p, int b, Seq *s)
+{
+    *s = sequence(p, min(b, p.batch - 1));
+    return b < p.batch ? (int64_t)tiles_of(p, *s) * p.kv_heads * blocks_of(*s) : 0;
+}
+// a value that all lanes share, in scalar registers (the vector ones are the inner loop's)
+__device__ __forceinline__ int64_t uniform(int64_t x) { return (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)x); }
+__device__ __forceinline__ int64_t wave_sum(int64_t x)
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor((long long)x, o, 64);
+    return uniform(x);
+}
+__device__ __forceinline__ int64_t all_blocks(const AttnParams &p)
+{
+    int64_t sum = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 64) {
+        Seq s;
+        sum += seq_blocks(p, b0 + (threadIdx.x & 63), &s);
+    }
+    return wave_sum(sum);
+}
+__device__ __forceinline__ int64_t share(const AttnParams &p, int64_t all) { return max((all + p.shares - 1) / p.shares, (int64_t)LEAST_BLOCKS); }
+
+// A place in the row of blocks: sequence, tile (of its heads' tiles, one head's after another), block
+struct Place {
+    int q0, nq, k0, nk, tiles, blocks, tile, block;
+};
+// the place `rest` blocks into the sequence that lane c holds
+__device__ __forceinline__ Place place(const AttnParams &p, const Seq &s, int c, int64_t rest)
+{
+    Place a;
+    a.q0 = __builtin_amdgcn_readlane(s.q0, c), a.nq = __builtin_amdgcn_readlane(s.nq, c);
+    a.k0 = __builtin_amdgcn_readlane(s.k0, c), a.nk = __builtin_amdgcn_readlane(s.nk, c);
+    a.tiles = __builtin_amdgcn_readlane(tiles_of(p, s), c), a.blocks = __builtin_amdgcn_readlane(blocks_of(s), c);
+    a.tile = __builtin_amdgcn_readfirstlane((int)(rest / a.blocks));
+    a.block = __builtin_amdgcn_readfirstlane((int)(rest - (int64_t)a.tile * a.blocks));
+    return a;
+}
+// blocks of the sequences from b0 on up to and with this lane's
+__device__ __forceinline__ int64_t scan_blocks(const AttnParams &p, int b0, Seq *s, int64_t *mine)
+{
+    const int lane = threadIdx.x & 63;
+    int64_t upto = *mine = seq_blocks(p, b0 + lane, s);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t x = __shfl_up((long long)upto, o, 64);
+        upto += lane >= o ? x : 0;
+    }
+    return upto;
+}
+__device__ __forceinline__ bool find_block(const AttnParams &p, int64_t u, Place *a)
+{
+    for (int b0 = 0; b0 < p.batch; b0 += 64) {
+        Seq s;
+        int64_t mine;
+        const int64_t upto = scan_blocks(p, b0, &s, &mine);
+        const int c = __popcll(__ballot(upto <= u));
+        if (c < 64) {
+            *a = place(p, s, c, u - uniform(__shfl((long long)(upto - mine), c, 64)));
+            return true;
+        }
+        u -= uniform(__shfl((long long)upto, 63, 64));
+    }
+    return false;
+}
+// where share i begins, and how many blocks a share has
+__device__ __forceinline__ bool find_share(const AttnParams &p, int i, Place *a, int64_t *per)
+{
+    if (p.batch > 64) {
+        *per = uniform(share(p, all_blocks(p)));
+        return find_block(p, i * *per, a);
+    }
+    Seq s;
+    int64_t mine;
+    const int64_t upto = scan_blocks(p, 0, &s, &mine), all = uniform(__shfl((long long)upto, 63, 64));
+    *per = uniform(share(p, all));
+    const int64_t u = i * *per;
+    if (u >= all) return false;
+    const int c = __popcll(__ballot(upto <= u));
+    *a = place(p, s, c, u - uniform(__shfl((long long)(upto - mine), c, 64)));
+    return true;
+}
+
 // ------------------------------------------------------------------------------------------------ tiles in the LDS
 // A tile is KT rows of DP values in row order; the 16-byte pieces of a row are permuted among themselves by a function of
 // the row so that the reads below meet different banks: K is read 16 bytes a lane, one piece of 32 rows at a time; V four
@@ -147,9 +241,8 @@ template <int DP, int KT, int WAVES, bool STREAM = false> struct Loader {
     static constexpr int PIECES = DP / 8, PER = KT * PIECES / 64 / WAVES;
     static_assert(PER >= 1, "every wavefront loads something");
     int off[PER];
-    __device__ __forceinline__ void init(int64_t stride, int dim, int wave, bool is_v)
+    __device__ __forceinline__ void init(int64_t stride, int dim, int lane, int wave, bool is_v)
     {
-        const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int at = (i * WAVES + wave) * 64 + lane, row = at / PIECES;
@@ -179,9 +272,9 @@ template <int T, int DP, int KT> struct Rows {
     int lim;         // last key this lane's row sees
     int k_at, v_at[DS];
 
-    __device__ __forceinline__ void init(const AttnParams &p, const Tile &t, int kv_head, int row, bool valid)
+    __device__ __forceinline__ void init(const AttnParams &p, const Tile &t, int kv_head, int row, bool valid, int lane)
     {
-        const int lane = threadIdx.x & 63, half = lane >> 5;
+        const int half = lane >> 5;
         const int i = row / p.group, head = kv_head * p.group + row - i * p.group;
         lim = t.nk - t.nq + i;
         const u16 *q = p.q + (int64_t)(t.q0 + i) * p.q_stride + (int64_t)head * p.dim + 8 * half;
@@ -332,13 +425,9 @@ template <int T, int DP, int KT> struct Rows {
 // this wavefront's loads into the LDS have landed and its reads are done, and so for the whole workgroup
 __device__ __forceinline__ void lds_arrived() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int T> __device__ __forceinline__ void write4(const AttnParams &p, const Tile &t, int kv_head, int row, int d, int split, f32x4 x)
+template <int T> __device__ __forceinline__ void write4(const AttnParams &p, const Tile &t, int kv_head, int row, int d, f32x4 x)
 {
     const int i = row / p.group, head = kv_head * p.group + row - i * p.group;
-    if (p.splits > 1) {
-        *reinterpret_cast<f32x4 *>(p.part_o + ((int64_t)split * p.total_q * p.q_heads + (int64_t)(t.q0 + i) * p.q_heads + head) * p.dim + d) = x;
-        return;
-    }
     u16x4 y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = narrow<T>(x[e]);
@@ -346,29 +435,21 @@ template <int T> __device__ __forceinline__ void write4(const AttnParams &p, con
 }
 
 // ------------------------------------------------------------------------------------------------ TILE: rows over wavefronts
-// Bound by the matrix units' feed: one prompt of 8192 tokens, 20 heads of 128 on 5, bf16: 344 GFLOP in 325 to 345 us, 1.0 to 1.06 PFLOP/s, where a
+// Bound by the matrix units' feed and the power it draws: one prompt of 8192 tokens, 20 heads of 128 on 5, bf16: 344 GFLOP in 325 to 345 us, 1.0 to 1.06 PFLOP/s, where a
 // product of two 8192 x 8192 matrices reaches 1.21 on the same card.  64 KB of LDS leave two workgroups to a compute unit, and
 // one's exponentials run beside the other's products; of the time, the exponentials alone are a tenth, the loads 3 %.  Four
 // wavefronts of 32 rows share each tile of K and V through the LDS (without bank conflicts); of 256 rows: slower, one workgroup a unit.
-template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) attention_tile_kernel(const AttnParams p)
+// Keys begin .. end - 1 (begin a multiple of the tile of keys, end one too or the last key that a row sees) for the 128 rows of t.
+// part < 0: the rows are done and written; else their sums become part `part` in the workspace.
+template <int T, int DP, int KT, int WAVES> __device__ __forceinline__ void tile_rows(const AttnParams &p, const Tile &t, int kv_head, int begin, int end, int i_last, char *k_a, char *k_b,
+                                                                                      char *v_a, char *v_b, int part)
 {
-    static_assert(WAVES == 4, "128 rows");
-    constexpr int LOG_TM = 7, TM = 1 << LOG_TM;
-    __shared__ __attribute__((aligned(1024))) char k_a[KT * DP * 2], k_b[KT * DP * 2], v_a[KT * DP * 2], v_b[KT * DP * 2];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    Tile t;
-    // A sequence's last rows, which see the most keys, first, and of all heads before the next rows: workgroups dispatched late
-    // are short.  (All sequences' tiles in one order of the keys they see: eight chunks of up to 400 tokens 361 us, so 371; thirty
-    // prompts of 30 to 1500 tokens 170, so 150.  Heads kept to their XCDs' L2s: one prompt of 8192, 5 heads, 341 and 346; 32 heads 524 and 510.)
-    const int kv_head = (int)(blockIdx.x % (unsigned)p.kv_heads), split = blockIdx.z, slot = p.slots - 1 - (int)(blockIdx.x / (unsigned)p.kv_heads);
-    if (!find_tile<LOG_TM>(p, slot, &t)) return;
-    const int i_last = (min(t.row0 + TM, t.rows) - 1) / p.group, all = min(t.nk, t.nk - t.nq + i_last + 1);
-    const int begin = split * p.chunk, end = split == p.splits - 1 ? all : min(all, begin + p.chunk);
-    if (split && begin >= end) return;
-
+    unsigned thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));  // (what follows from it is computed here and not kept in registers from one call to the next)
+    const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     Loader<DP, KT, WAVES> lk, lv;
-    lk.init(p.k_stride, p.dim, wave, false);
-    lv.init(p.v_stride, p.dim, wave, true);
+    lk.init(p.k_stride, p.dim, lane, wave, false);
+    lv.init(p.v_stride, p.dim, lane, wave, true);
     const u16 *k = p.k + (int64_t)t.k0 * p.k_stride + (int64_t)kv_head * p.dim, *v = p.v + (int64_t)t.k0 * p.v_stride + (int64_t)kv_head * p.dim;
 
     const int n = begin < end ? (end - begin + KT - 1) / KT : 0;
@@ -385,7 +466,7 @@ template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64
     R r;
     const int row = t.row0 + wave * 32 + (lane & 31);
     const bool valid = row < t.rows;
-    r.init(p, t, kv_head, valid ? row : t.rows - 1, valid);
+    r.init(p, t, kv_head, valid ? row : t.rows - 1, valid, lane);
     const int row_w = t.row0 + wave * 32, lo = t.nk - t.nq + row_w / p.group;
     const int hi = row_w < t.rows ? t.nk - t.nq + min(i_last, (row_w + 31) / p.group) : -1;
     int i = 0;
@@ -409,9 +490,10 @@ template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64
         if (j <= hi) r.template step<R::EDGE>(p, k_b, v_b, j, lo, r.polluted(v_b, j, end, lo));
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing is on its way into the LDS when the workgroup gives it up)
-    const float sum = halves_sum(r.sum), f = p.splits > 1 ? 1.f : 1.f / sum;
+    const float sum = halves_sum(r.sum), f = part < 0 ? 1.f / sum : 1.f;
     if (!valid) return;
     const bool none = r.lim < 0;
+    const int64_t part_row = (int64_t)part * (32 * WAVES) + row - t.row0;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -420,11 +502,43 @@ template <int T, int DP, int KT, int WAVES> __global__ void __launch_bounds__(64
             f32x4 x;
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = none ? 0.f : r.o[d][4 * e + i] * f;
-            if (at < p.dim) write4<T>(p, t, kv_head, row, at, split, x);
+            if (at >= p.dim) continue;
+            if (part < 0) write4<T>(p, t, kv_head, row, at, x);
+            else *reinterpret_cast<f32x4 *>(p.part_o + part_row * p.dim + at) = x;
         }
-    if (p.splits > 1 && lane < 32) {
-        const int i = row / p.group, head = kv_head * p.group + row - i * p.group;
-        p.part_ml[(int64_t)split * p.total_q * p.q_heads + (int64_t)(t.q0 + i) * p.q_heads + head] = float2{r.top, sum};
+    if (part >= 0 && lane < 32) p.part_ml[part_row] = float2{r.top, sum};
+}
+
+// SHARED: the blocks of keys of all tiles, tile after tile, are cut into equal shares, one a workgroup; a share may end within a tile
+// and go on in the next.  A tile that lies in one share is written; others leave their sums, a workgroup at most two: of a
+// tile that it ends (part 0) and of one that it begins (part 1).  Neighbouring shares, which read the same keys, go to one XCD.
+template <int T, int DP, int KT, int WAVES, bool SHARED> __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) attention_tile_kernel(const AttnParams p)
+{
+    __shared__ __attribute__((aligned(1024))) char k_a[KT * DP * 2], k_b[KT * DP * 2], v_a[KT * DP * 2], v_b[KT * DP * 2];
+    Tile t;
+    if constexpr (SHARED) {
+        const int i = (int)(blockIdx.x % 8 * (p.shares / 8) + blockIdx.x / 8);
+        Place a;
+        int64_t per;
+        if (!find_share(p, i, &a, &per)) return;
+        for (int64_t left = per;;) {
+            const int kv_head = a.tile / a.tiles, n = (int)min((int64_t)(a.blocks - a.block), left);
+            t = {a.q0, a.nq, a.k0, a.nk, (a.tile - kv_head * a.tiles) << p.log_rows, a.nq * p.group};
+            const int i_last = (min(t.row0 + 32 * WAVES, t.rows) - 1) / p.group, all = max(0, min(t.nk, t.nk - t.nq + i_last + 1));
+            tile_rows<T, DP, KT, WAVES>(p, t, kv_head, min(a.block << LOG_BLOCK, all), min((a.block + n) << LOG_BLOCK, all), i_last, k_a, k_b, v_a, v_b, n == a.blocks ? -1 : 2 * i + (a.block == 0));
+            if ((left -= n) == 0) return;
+            a.block = 0;
+            if (++a.tile == a.tiles * p.kv_heads && !find_block(p, (i + 1) * per - left, &a)) return;
+            __syncthreads();  // (all are done with the tiles of keys)
+        }
+    } else {
+        // A sequence's last rows, which see the most keys, first, and of all heads before the next rows: workgroups dispatched late
+        // are short.  (All sequences' tiles in one order of the keys they see: eight chunks of up to 400 tokens 361 us, so 371; thirty
+        // prompts of 30 to 1500 tokens 170, so 150.  Heads kept to their XCDs' L2s: one prompt of 8192, 5 heads, 341 and 346; 32 heads 524 and 510.)
+        const int kv_head = (int)(blockIdx.x % (unsigned)p.kv_heads), slot = p.slots - 1 - (int)(blockIdx.x / (unsigned)p.kv_heads);
+        if (!find_tile<LOG_TILE>(p, slot, &t)) return;
+        const int i_last = (min(t.row0 + TILE_ROWS, t.rows) - 1) / p.group, all = min(t.nk, t.nk - t.nq + i_last + 1);
+        tile_rows<T, DP, KT, WAVES>(p, t, kv_head, 0, all, i_last, k_a, k_b, v_a, v_b, -1);
     }
 }
 
@@ -446,8 +560,8 @@ template <int T, int DP, int WAVES, bool STREAM> __global__ void __launch_bounds
     if (split && begin >= end) return;
 
     Loader<DP, KT, 1, STREAM> lk, lv;
-    lk.init(p.k_stride, p.dim, 0, false);
-    lv.init(p.v_stride, p.dim, 0, true);
+    lk.init(p.k_stride, p.dim, lane, 0, false);
+    lv.init(p.v_stride, p.dim, lane, 0, true);
     const u16 *k = p.k + (int64_t)t.k0 * p.k_stride + (int64_t)kv_head * p.dim, *v = p.v + (int64_t)t.k0 * p.v_stride + (int64_t)kv_head * p.dim;
     // this wavefront's tiles: every WAVES-th, one in use while the next is on its way
     constexpr int STRIDE = WAVES * KT;
@@ -469,7 +583,7 @@ template <int T, int DP, int WAVES, bool STREAM> __global__ void __launch_bounds
     load(0, k_a, v_a);
     R r;
     const bool valid = (lane & 31) < rows;
-    r.init(p, t, kv_head, t.row0 + (valid ? lane & 31 : 0), valid);
+    r.init(p, t, kv_head, t.row0 + (valid ? lane & 31 : 0), valid, lane);
     int i = 0;
     for (; i < clean; i += 2) {
         load(i + 1, k_b, v_b);
@@ -521,79 +635,62 @@ template <int T, int DP, int WAVES, bool STREAM> __global__ void __launch_bounds
         for (int w = 0; w < WAVES; ++w) total += tops[w][rr] == -INFINITY ? 0.f : sums[w][rr] * __builtin_amdgcn_exp2f((tops[w][rr] - best) * p.c);
         const int row = t.row0 + rr, i = row / p.group;
         if (p.splits > 1) {
-            if (d4 == 0)
-                p.part_ml[(int64_t)split * p.total_q * p.q_heads + (int64_t)(t.q0 + i) * p.q_heads + kv_head * p.group + row - i * p.group] = float2{best, total};
+            const int64_t part_row = (int64_t)split * p.total_q * p.q_heads + (int64_t)(t.q0 + i) * p.q_heads + kv_head * p.group + row - i * p.group;
+            if (d4 == 0) p.part_ml[part_row] = float2{best, total};
+            *reinterpret_cast<f32x4 *>(p.part_o + part_row * p.dim + 4 * d4) = x;
         } else {
             const float inv = 1.f / total;
             const bool none = t.nk - t.nq + i < 0;
 #pragma unroll
             for (int c = 0; c < 4; ++c) x[c] = none ? 0.f : x[c] * inv;
+            write4<T>(p, t, kv_head, row, 4 * d4, x);
         }
-        write4<T>(p, t, kv_head, row, 4 * d4, split, x);
     }
 }
 
-// ------------------------------------------------------------------------------------------------ splits joined
-// Per (query, head) the splits that hold keys the row sees, added in a fixed order, by WAVES wavefronts: the four of a workgroup
-// where there are many splits (one token of 20 heads against 8000 keys, 63 splits: the call 13.6 us, by single wavefronts
-// 16.8), one where there are few and many rows (870 x 20 rows of four: 204 us, by four wavefronts each 217).
-template <int T, int WAVES> __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
+// ------------------------------------------------------------------------------------------------ parts joined
+// One row's n parts, added in their order by WAVES wavefronts and written: the four of a workgroup where there are many parts
+// (one token of 20 heads against 8000 keys, 63 parts: the call 13.6 us, by single wavefronts 16.8), one where there are few
+// and many rows.  at(i): where part i lies.
+template <int T, int WAVES, int MOST, typename At> __device__ __forceinline__ void join_row(const AttnParams &p, f32x4 (&parts)[4][64], int wave, int n, bool none, At at, u16 *out)
 {
-    __shared__ __attribute__((aligned(16))) f32x4 parts[4][64];
-    const int lane = threadIdx.x & 63, in_block = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = WAVES == 1 ? 0 : in_block;
-    const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + in_block : blockIdx.x, all = (int64_t)p.total_q * p.q_heads;
-    if (row >= all) return;
-    const int query = (int)(row / p.q_heads), head = (int)(row - (int64_t)query * p.q_heads);
-    // the sequence of this query: the last one that starts at or before it
-    Seq s = {0, 0, 0, 0};
-    for (int b0 = 0; b0 < p.batch; b0 += 64) {
-        const int b = b0 + lane;
-        const Seq mine = sequence(p, min(b, p.batch - 1));
-        const int c = __popcll(__ballot(b < p.batch && mine.q0 <= query));
-        if (c == 0) break;
-        s = {__builtin_amdgcn_readlane(mine.q0, c - 1), __builtin_amdgcn_readlane(mine.nq, c - 1), 0, __builtin_amdgcn_readlane(mine.nk, c - 1)};
-        if (c < 64) break;
-    }
-    if (query >= s.q0 + s.nq) return;  // a row behind the last sequence
-    const int seen = s.nk - s.nq + (query - s.q0) + 1;
-    const int n = seen <= 0 ? 0 : min(p.splits, (seen + p.chunk - 1) / p.chunk);
-    // every lane holds the weight of one split (and of those 64, 128 and 192 further)
-    float2 ml[4];
+    constexpr int PER = MOST / 64;
+    const int lane = threadIdx.x & 63;
+    // every lane holds the weight of one part (and of those 64, 128, ... further)
+    float2 ml[PER];
     float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        ml[i] = lane + 64 * i < n ? p.part_ml[(lane + 64 * i) * all + row] : float2{-INFINITY, 0.f};
+    for (int i = 0; i < PER; ++i) {
+        ml[i] = lane + 64 * i < n ? p.part_ml[at(lane + 64 * i)] : float2{-INFINITY, 0.f};
         top = fmaxf(top, ml[i].x);
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    float w[4];
+    float w[PER];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < PER; ++i) {
         w[i] = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i].x - top) * p.c);
         sum = fmaf(ml[i].y, w[i], sum);
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-    // four values a lane, and as many splits side by side as lanes are left, and every WAVES-th such group a wavefront's
+    // four values a lane, and as many parts side by side as lanes are left, and every WAVES-th such group a wavefront's
     const int quads = p.dim / 4, log_l = quads <= 2 ? 1 : 32 - __builtin_clz(quads - 1), sub = lane >> log_l, d4 = lane & ((1 << log_l) - 1), step = 64 >> log_l;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < PER; ++i) {
         const int end = min(64, n - 64 * i);
         for (int s0 = wave * step; s0 < end; s0 += 4 * WAVES * step) {
             f32x4 x[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {  // (four loads in flight; behind the last split: its values, times zero)
-                const int at = min(64 * i + s0 + u * WAVES * step + sub, n - 1);
-                x[u] = *reinterpret_cast<const f32x4 *>(p.part_o + (at * all + row) * p.dim + 4 * min(d4, quads - 1));
-            }
+            for (int u = 0; u < 4; ++u)  // (four loads in flight; behind the last part: its values, left out below)
+                x[u] = *reinterpret_cast<const f32x4 *>(p.part_o + at(min(64 * i + s0 + u * WAVES * step + sub, n - 1)) * p.dim + 4 * min(d4, quads - 1));
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int at = s0 + u * WAVES * step + sub;
-                const float f = __shfl(w[i], at & 63, 64);
+                const int s = s0 + u * WAVES * step + sub;
+                const float f = __shfl(w[i], s & 63, 64);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = at < end ? fmaf(x[u][e], f, o[e]) : o[e];
+                for (int e = 0; e < 4; ++e) o[e] = s < end ? fmaf(x[u][e], f, o[e]) : o[e];
             }
         }
     }
@@ -609,8 +706,49 @@ template <int T, int WAVES> __global__ void __launch_bounds__(256) attention_joi
     const float inv = 1.f / sum;
     u16x4 y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = narrow<T>(n ? o[e] * inv : 0.f);
-    *reinterpret_cast<u16x4 *>(p.out + (int64_t)query * p.out_stride + (int64_t)head * p.dim + 4 * d4) = y;
+    for (int e = 0; e < 4; ++e) y[e] = narrow<T>(none ? 0.f : o[e] * inv);
+    *reinterpret_cast<u16x4 *>(out + 4 * d4) = y;
+}
+
+// Per (query, head).  SHARED: the parts that the shares left of the row's tile, if they cut it; else the splits that hold keys the row sees.
+template <int T, int WAVES, bool SHARED> __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
+{
+    __shared__ __attribute__((aligned(16))) f32x4 parts[4][64];
+    const int lane = threadIdx.x & 63, in_block = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = WAVES == 1 ? 0 : in_block;
+    const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + in_block : blockIdx.x, all = (int64_t)p.total_q * p.q_heads;
+    if (row >= all) return;
+    const int query = (int)(row / p.q_heads), head = (int)(row - (int64_t)query * p.q_heads);
+    // the sequence of this query: the last one that starts at or before it; the blocks before it, and all
+    Seq s = {0, 0, 0, 0};
+    int64_t before = 0, blocks = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 64) {
+        const int b = b0 + lane;
+        Seq mine;
+        int64_t w = 0;
+        if constexpr (SHARED) w = seq_blocks(p, b, &mine);
+        else mine = sequence(p, min(b, p.batch - 1));
+        const int c = __popcll(__ballot(b < p.batch && mine.q0 <= query));
+        if (c) {
+            s = {__builtin_amdgcn_readlane(mine.q0, c - 1), __builtin_amdgcn_readlane(mine.nq, c - 1), 0, __builtin_amdgcn_readlane(mine.nk, c - 1)};
+            before = blocks + (lane < c - 1 ? w : 0);
+        }
+        blocks += w;
+        if (!SHARED && c < 64) break;
+    }
+    if (query >= s.q0 + s.nq) return;  // a row behind the last sequence
+    u16 *const out = p.out + (int64_t)query * p.out_stride + (int64_t)head * p.dim;
+    const int seen = s.nk - s.nq + (query - s.q0) + 1;
+    if constexpr (SHARED) {
+        const int64_t per = share(p, wave_sum(blocks));
+        const int kv_head = head / p.group, r = (query - s.q0) * p.group + head - kv_head * p.group, mine = blocks_of(s);
+        const int64_t first = wave_sum(before) + ((int64_t)kv_head * tiles_of(p, s) + (r >> p.log_rows)) * mine;
+        const int i0 = (int)min(first / per, (int64_t)p.shares - 1), i1 = (int)min((first + mine - 1) / per, (int64_t)p.shares - 1);
+        if (i0 == i1) return;  // written already
+        join_row<T, WAVES, MOST_SHARES>(p, parts, wave, i1 - i0 + 1, seen <= 0, [&](int i) { return ((int64_t)(2 * (i0 + i) + (i == 0)) << p.log_rows) + (r & ((1 << p.log_rows) - 1)); }, out);
+    } else {
+        const int n = seen <= 0 ? 0 : min(p.splits, (seen + p.chunk - 1) / p.chunk);
+        join_row<T, WAVES, 256>(p, parts, wave, n, n == 0, [&](int i) { return i * all + row; }, out);
+    }
 }
 
 int check(const sptmm_attention_args *a)
@@ -632,63 +770,84 @@ int check(const sptmm_attention_args *a)
 struct Cut {
     bool keys;  // the KEYS form
     bool stream;
-    int dp, slots, splits, chunk;
+    int dp, slots, splits, chunk, shares, log_rows;
 };
-
 Cut cut(const sptmm_attention_args *a)
 {
     Cut c{};
     const int group = a->q_heads / a->kv_heads;
     c.dp = a->head_dim <= 64 ? 64 : a->head_dim <= 128 ? 128 : 256;
     c.keys = (int64_t)a->max_q * group <= 32;
-    const int tm = c.keys ? 32 : 128;
+    const int tm = c.keys ? 32 : TILE_ROWS;
     const int64_t rows = (int64_t)a->total_q * group;
     c.slots = (int)(rows / tm + a->batch);
-    // Workgroups without splits (those that have rows): about as many as sequences have tiles.  Splits where they are fewer than
-    // the chip has places for -- two per compute unit, of the TILE form with heads of 256 one --, in the TILE form three quarters
-    // of that: 512 tokens against 16000 keys, 8 heads: 113 us, with all the places 134; eight chunks of 64 tokens against 3000
-    // to 9000, 5 heads: 67 and 75; four chunks of 130 to 250 against 12000 to 20000, 5 heads: 214 and 200.
+    // workgroups of one tile each (those that have rows): about as many as sequences have tiles
     const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>(c.slots, c.keys ? (int64_t)a->batch : rows / tm + 1)) * a->kv_heads;
-    const int64_t room = c.keys ? 512 : c.dp == 256 ? 192 : 384;
     const int max_kv = (int)std::min<int64_t>(a->max_kv, a->kv_rows);
-    // Keys a workgroup should have at least.  Where the queries are most of the keys, half the tiles see little of a late split
-    // and the join has many rows: one prompt of 600, 1024, 1500 tokens, 20 heads on 5: 19, 25, 35 us at 2048, 27, 32, 48 at 512
-    // (2000 tokens, 8 heads on 2: 40 and 36).  A chunk of 64 against 1500, of 200 against 2000: 32, 41 us at 2048, 21, 25 at 512.
-    const int unit = c.keys ? 128 : 2ll * a->max_q >= max_kv ? 2048 : 512;
-    const int64_t want = (room + tiles - 1) / tiles, most = (max_kv + unit - 1) / unit;
-    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
-    if ((int64_t)a->total_q * a->q_heads >= (1 << 24)) c.splits = 1;  // (one launch of the join holds fewer rows)
-    c.chunk = std::max(unit, (max_kv / c.splits + 127) / 128 * 128);
-    c.splits = std::max(1, std::min(c.splits, (max_kv + c.chunk - 1) / c.chunk));
+    c.splits = 1;
+    if ((int64_t)a->total_q * a->q_heads >= (1 << 24)) {
+        // (one launch of the join holds fewer rows)
+    } else if (c.keys) {
+        // Splits where these are fewer than the chip has places for, two per compute unit.
+        const int unit = 128;  // keys a workgroup should have at least
+        const int64_t want = (512 + tiles - 1) / tiles, most = (max_kv + unit - 1) / unit;
+        c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
+        c.chunk = std::max(unit, (max_kv / c.splits + 127) / 128 * 128);
+        c.splits = std::max(1, std::min(c.splits, (max_kv + c.chunk - 1) / c.chunk));
+    } else {
+        // Shares instead of a workgroup per tile where there are too few tiles to fill the chip evenly.  Heads of 128, bf16: four chunks
+        // of 130 to 250 tokens against 12000 to 20000, 5 heads (140 tiles): shares 182 us, tiles 345; eight of 400 against 1400 to 20000
+        // (400 tiles) 340 and 385; eight of 300 against 9000, 32 heads (480) 389 and 361; sixteen of 512 against 12000 (960) 629 and
+        // 607.  Where the queries are most of the keys tiles see half of theirs, and shares are less equal: 4096 tokens, 1 head of a
+        // group of 4 (129) 55 and 69, 3000 tokens, 2 heads (188) 67 and 55, 2000 tokens (126) 45 and 38.
+        // Tiles of 256 rows, a workgroup per compute unit, read the keys half as often: one chunk of 161 tokens against 60000 135 us, of
+        // 128 rows 157; they are left to work that fills them (200 tokens against 2000: 31 and 25).  A share of two blocks at
+        // least: 64 tokens against 1500 18.9 us, of four 22.0.
+        const bool chunks = 4ll * a->max_q < max_kv;
+        if (tiles < (chunks ? 448 : 160) && max_kv > (chunks ? 512 : 2048)) {
+            const int64_t shares = (int64_t)c.slots * a->kv_heads * ((max_kv >> LOG_BLOCK) + 1) / LEAST_BLOCKS;
+            c.log_rows = c.dp == 256 || shares < MOST_SHARES ? 7 : 8;
+            c.shares = (int)std::min<int64_t>(c.dp == 256 || c.log_rows == 8 ? 256 : MOST_SHARES, (shares + 7) / 8 * 8);
+        }
+    }
     // Caches that no level below holds between two calls are read past them: 661 MB 120 us (5.5 TB/s), through them 133; 246 MB 55
     // and 61.  Below, no way wins: 123 MB 33.8 and 35.9, 33 MB 14.3 and 13.6.
     c.stream = (int64_t)a->batch * max_kv * a->kv_heads * a->head_dim * 4 > (128ll << 20);
     return c;
 }
 
-size_t workspace(const sptmm_attention_args *a, const Cut &c)
-{
-    if (c.splits <= 1) return 0;
-    const size_t rows = (size_t)a->total_q * a->q_heads * c.splits;
-    return (rows * a->head_dim * 4 + 255) / 256 * 256 + rows * 8;
-}
+// rows of parts in the workspace
+int64_t part_rows(const sptmm_attention_args *a, const Cut &c) { return c.shares ? 2ll * c.shares << c.log_rows : c.splits > 1 ? (int64_t)a->total_q * a->q_heads * c.splits : 0; }
+size_t part_bytes(const sptmm_attention_args *a, const Cut &c) { return ((size_t)part_rows(a, c) * a->head_dim * 4 + 255) / 256 * 256; }
+size_t workspace(const sptmm_attention_args *a, const Cut &c) { return part_bytes(a, c) + (size_t)part_rows(a, c) * 8; }
 
+template <int T, int DP, int KT> void launch_tiles(const AttnParams &p, hipStream_t st)
+{
+    if (p.shares && p.log_rows == 8) {
+        if constexpr (DP <= 128) hipLaunchKernelGGL((attention_tile_kernel<T, DP, KT, 8, true>), dim3(p.shares), dim3(512), 0, st, p);
+    } else if (p.shares) hipLaunchKernelGGL((attention_tile_kernel<T, DP, KT, 4, true>), dim3(p.shares), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((attention_tile_kernel<T, DP, KT, 4, false>), dim3((unsigned)p.slots * p.kv_heads), dim3(256), 0, st, p);
+}
+template <int T, bool SHARED> void launch_join(const AttnParams &p, bool many, hipStream_t st)
+{
+    if (many) hipLaunchKernelGGL((attention_join_kernel<T, 4, SHARED>), dim3((unsigned)(p.total_q * p.q_heads)), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((attention_join_kernel<T, 1, SHARED>), dim3((unsigned)((p.total_q * p.q_heads + 3) / 4)), dim3(256), 0, st, p);
+}
 template <int T> void launch(const AttnParams &p, const Cut &c, hipStream_t st)
 {
-    const dim3 grid = c.keys ? dim3(c.slots, p.kv_heads, c.splits) : dim3((unsigned)c.slots * p.kv_heads, 1, c.splits);
     if (c.keys) {
+        const dim3 grid(c.slots, p.kv_heads, c.splits);
         const auto kernel = c.dp == 64    ? (c.stream ? attention_keys_kernel<T, 64, 2, true> : attention_keys_kernel<T, 64, 2, false>)
                             : c.dp == 128 ? (c.stream ? attention_keys_kernel<T, 128, 2, true> : attention_keys_kernel<T, 128, 2, false>)
                                           : (c.stream ? attention_keys_kernel<T, 256, 2, true> : attention_keys_kernel<T, 256, 2, false>);
         hipLaunchKernelGGL(kernel, grid, dim3(128), 0, st, p);
-    } else {
-        if (c.dp == 64) hipLaunchKernelGGL((attention_tile_kernel<T, 64, 64, 4>), grid, dim3(256), 0, st, p);
-        else if (c.dp == 128) hipLaunchKernelGGL((attention_tile_kernel<T, 128, 64, 4>), grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((attention_tile_kernel<T, 256, 32, 4>), grid, dim3(256), 0, st, p);
+        if (c.splits > 1) launch_join<T, false>(p, c.splits > 8, st);
+        return;
     }
-    if (c.splits <= 1) return;
-    if (c.splits > 8) hipLaunchKernelGGL((attention_join_kernel<T, 4>), dim3((unsigned)(p.total_q * p.q_heads)), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((attention_join_kernel<T, 1>), dim3((unsigned)((p.total_q * p.q_heads + 3) / 4)), dim3(256), 0, st, p);
+    if (c.dp == 64) launch_tiles<T, 64, 64>(p, st);
+    else if (c.dp == 128) launch_tiles<T, 128, 64>(p, st);
+    else launch_tiles<T, 256, 32>(p, st);
+    if (c.shares) launch_join<T, true>(p, c.shares > 8ll * (p.total_q * (int64_t)p.group / TILE_ROWS + 1) * p.kv_heads, st);
 }
 
 }  // namespace
@@ -724,10 +883,9 @@ extern "C" int sptmm_attention(const sptmm_attention_args *a, void *workspace_de
     p.q_start = a->q_start, p.kv_start = a->kv_start, p.kv_len = a->kv_len;
     p.batch = a->batch, p.total_q = a->total_q, p.q_heads = a->q_heads, p.kv_heads = a->kv_heads, p.group = a->q_heads / a->kv_heads, p.dim = a->head_dim;
     p.c = a->scale * 1.44269504088896340736f;
-    p.slots = c.slots, p.splits = c.splits, p.chunk = c.chunk;
+    p.slots = c.slots, p.splits = c.splits, p.chunk = c.chunk, p.shares = c.shares, p.log_rows = c.log_rows;
     p.part_o = (float *)workspace_dev;
-    const size_t o_bytes = ((size_t)a->total_q * a->q_heads * c.splits * a->head_dim * 4 + 255) / 256 * 256;
-    p.part_ml = want ? (float2 *)((char *)workspace_dev + o_bytes) : nullptr;
+    p.part_ml = want ? (float2 *)((char *)workspace_dev + part_bytes(a, c)) : nullptr;
     a->type == SPTMM_X_F16 ? launch<SPTMM_X_F16>(p, c, (hipStream_t)stream) : launch<SPTMM_X_BF16>(p, c, (hipStream_t)stream);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? SPTMM_OK : fail(SPTMM_ERR_HIP, "attention kernels launch: %s (%d)", hipGetErrorString(e), (int)e);

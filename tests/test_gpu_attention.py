@@ -121,6 +121,33 @@ def test_chunks_of_prompts_against_longer_and_shorter_caches(dim):
     one(9, [3, 5, 0, 2], [300, 4, 10, 2], (8, 2), dim, "f16")
 
 
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [40, 128, 256])
+def test_equal_shares_of_unequal_chunks(dim, t):
+    """Shares that end within a tile, shares of several short tiles, rows that see nothing of a part or nothing at all."""
+    one(30, [40, 130, 0, 9, 1, 300], [3000, 20, 500, 0, 5000, 1700], (6, 2), dim, t, tail=2, pad=8)
+
+
+def test_equal_shares_of_many_sequences_and_of_one_tile():
+    r = np.random.default_rng(31)
+    one(31, [int(x) for x in r.integers(0, 20, 150)], [int(x) for x in r.integers(0, 1500, 150)], (8, 1), 64, "bf16")
+    one(32, [9], [40000], (4, 1), 64, "f16")  # 79 parts
+
+
+@pytest.mark.parametrize("nq,nk,heads", [([2100, 300], [2100, 300], (2, 1)), ([900, 900], [2300, 2049], (3, 3)), ([513], [513], (4, 4))])
+def test_equal_shares_of_prompts(nq, nk, heads):
+    one(33, nq, nk, heads, 64, "f16", max_kv=5000)
+
+
+@pytest.mark.parametrize("what", [np.inf, np.nan])
+def test_what_is_not_finite_stays_with_its_rows_across_shares(what):
+    def edit(c, q, k, v):
+        v[c.kv_start[0] + 1990, 0, 3] = what  # seen by the last rows of the first sequence only
+        k[c.kv_start[1] + 1995, 1] = what
+
+    one(34, [60, 50], [2000, 2000], (4, 2), 64, "bf16", edit=edit)
+
+
 def test_rows_strides_and_gaps():
     one(10, [5, 60], [40, 77], (4, 2), 64, "f16", pad=8, tail=4)
     one(11, [1, 1], [400, 77], (4, 2), 128, "bf16", pad=24, tail=4)
