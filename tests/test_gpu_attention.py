@@ -284,3 +284,43 @@ def test_lengths_that_lead_out_of_the_buffers_are_cut():
     c.run()
     c.free()
     one(32, [4, 4], [20, 20], (4, 2), 64, "f16")
+
+
+def test_a_captured_call_of_shares_follows_its_lengths():
+    """How the work is shared out is found on the device: a replay with other lengths gives what a fresh call gives."""
+    st = sp.Stream()
+    c = Call(40, [60, 90, 20], [1500, 700, 40], (6, 2), 128, "bf16", max_kv=2500, gap=1200, max_q=120)
+    n = sp.attention_workspace_bytes(c.args)
+    assert n > 0
+    c.ws = sp.DeviceBuffer(n + 256)
+    with sp.Graph(st) as g:
+        sp.attention(c.args, c.ws, n, st)
+    for rep, (first, length) in enumerate((([0, 60, 150, 170], [2400, 700, 0]), ([0, 1, 120, 170], [3, 1900, 900]), ([0, 0, 170, 170], [0, 650, 5]))):
+        print("replay", rep, flush=True)
+        c.q_start, c.kv_len = np.array(first, np.int32), np.array(length, np.int32)
+        c.bufs[3].upload(c.q_start)
+        c.bufs[5].upload(c.kv_len)
+        c.ws.fill(0xFF)
+        g.launch(st)
+        st.sync()
+        c.got = got = c.out.to_numpy(np.uint16, c.before.shape)
+        c.check()
+        c.out.upload(c.before)
+        sp.attention(c.args, c.ws, n, st)
+        st.sync()
+        assert (c.out.to_numpy(np.uint16, c.before.shape) == got).all()
+    g.destroy()
+    c.free()
+    st.destroy()
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_shares_of_lengths_that_lead_out_of_the_buffers(dim):
+    c = Call(41, [90, 60, 70], [2000, 900, 20], (6, 2), dim, "f16", tail=2)
+    assert sp.attention_workspace_bytes(c.args) > 0
+    c.bufs[3].upload(np.array([0, 200, 3, 1 << 30], np.int32))
+    c.bufs[4].upload(np.array([-5, 1 << 30, 40], np.int32))
+    c.bufs[5].upload(np.array([1 << 30, 10, 1 << 30], np.int32))
+    c.run()
+    c.free()
+    one(42, [4, 4], [20, 20], (4, 2), 64, "f16")
