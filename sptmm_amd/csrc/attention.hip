@@ -17,7 +17,8 @@
 // Unnormalised sums and statistics of parts go to a workspace, and attention_join_kernel adds them up in their order.
 //
 // Rounding: products of 16-bit values summed in 32 bits; statistics, sums and rescaling in 32 bits; p is rounded to 16 bits
-// for the second product (half a step of p each, bf16 2^-8 and fp16 2^-11 of it: the terms' errors average out), the result once.
+// for the second product (half a step of p each, bf16 2^-8 and fp16 2^-11 of it: the terms' errors average out) and for the sum of
+// weights that divides it, the result once.
 // The maximum is followed only where weights relative to the last one outgrow 2^15: most tiles look for none and rescale nothing.
 #include <cmath>
 
@@ -63,6 +64,14 @@ template <int T> __device__ __forceinline__ u16 narrow(float x)
 {
     if constexpr (T == SPTMM_X_F16) return __builtin_bit_cast(u16, (_Float16)x);
     return __builtin_bit_cast(u16, (__bf16)x);
+}
+// the two values of a word added to a 32-bit sum
+template <int T> __device__ __forceinline__ float add_two(unsigned x, float sum)
+{
+    typedef __attribute__((ext_vector_type(2))) _Float16 h2;
+    typedef __attribute__((ext_vector_type(2))) __bf16 b2;
+    if constexpr (T == SPTMM_X_F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, x), h2{(_Float16)1.f, (_Float16)1.f}, sum, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, x), b2{(__bf16)1.f, (__bf16)1.f}, sum, false);
 }
 // a lane's value and that of the lane 32 further (mod 64)
 struct Halves {
@@ -355,18 +364,41 @@ template <int T, int DP, int KT> struct Rows {
             }
         };
         u16x8 pf[2 * KB];
-        // the weights relative to `top`, rounded into pf; their 32-bit sum.  fp16: p is held 2^7 larger, so that what rounds to zero is
-        // below 2^-32 of the largest.
+        // the weights relative to `top`, rounded into pf; their 32-bit sum, of the rounded values: a row of one key is then that key's value
+        // exactly, and a few keys' roundings cancel.  fp16: p is held 2^7 larger, so that what rounds to zero is below 2^-32 of
+        // the largest.
         auto weigh = [&] {
             const float at = (top == -INFINITY ? 0.f : top * p.c) - (T == SPTMM_X_F16 ? 7.f : 0.f);
             float part[4] = {0.f, 0.f, 0.f, 0.f};
+            // Summed behind all exponentials, or (heads of 256, one wavefront per SIMD) each pair at once: 3000 tokens of 256 169 us and 110,
+            // 8192 of 128 339 and 349.  (Sums of the weights before their rounding: 129 and 329, now 330, chunks 175 and 182.)
 #pragma unroll
-            for (int b = 0; b < KB; ++b)
+            for (int t = 0; t < 2 * KB; ++t) {
+                auto weight = [&](int e) { return __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + e], p.c, -at)); };
+                if constexpr (DP == 256) {
+                    u32x4 w;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[b][e], p.c, -at));
-                    part[e & 3] += x;
-                    pf[2 * b + (e >> 3)][e & 7] = narrow<T>(x);
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = weight(2 * i), y = weight(2 * i + 1);
+                        const unsigned two = narrow<T>(x) | (unsigned)narrow<T>(y) << 16;
+                        w[i] = two;
+                        part[i] = add_two<T>(two, part[i]);
+                    }
+                    pf[t] = __builtin_bit_cast(u16x8, w);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) pf[t][e] = narrow<T>(weight(e));
+                }
+            }
+            if constexpr (DP != 256)
+#pragma unroll
+                for (int t = 0; t < 2 * KB; ++t) {
+                    const u32x4 w = __builtin_bit_cast(u32x4, pf[t]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned two = w[i];
+                        part[i & 1] = add_two<T>(two, part[i & 1]);
+                    }
                 }
             return (part[0] + part[1]) + (part[2] + part[3]);
         };

@@ -74,7 +74,8 @@ def rotate_norm(x, pos, gain, eps, freq, interleaved, t):
 def attention(q, k, v, q_start, kv_start, kv_len, scale, t):
     """q [Tq][Hq][D], k and v [rows][Hkv][D] in 64 bits -> {row: (out [Hq][D], bound)} for the rows of the sequences.
 
-    The bound, A = sum p |v| / sum p being an output's mean magnitude: p is rounded to t (half a step of p each, so half a step of A);
+    The bound, A = sum p |v| / sum p being an output's mean magnitude: p is rounded to t, p (1 + d), in the numerator and in the
+    denominator, which moves o by sum p d (v - o) / sum p: half a step of sum p |v - o| / sum p;
     a score's 32-bit sum of D products and its scaling are off by (D + 8) 2^-23 of scale * sum |q||k|, which moves p by as
     much relatively, in the numerator and in the denominator; the exponential and the sums over n keys in 32 bits add (n + 64) 2^-23;
     fp16 loses p below 2^-32 of the largest, 2^-31 of sum |v| at most; the result is rounded once."""
@@ -93,10 +94,10 @@ def attention(q, k, v, q_start, kv_start, kv_len, scale, t):
                         p = np.exp(s - s.max())
                         p /= p.sum()
                         o[h] = p @ V
-                        A = p @ np.abs(V)
+                        A, spread = p @ np.abs(V), p @ np.abs(V - o[h])
                         some = np.isfinite(s)
                         ds = scale * (np.abs(K[some]) @ np.abs(Q)).max(initial=0.0) * (q.shape[2] + 8) * 2.0 ** -23
-                        e[h] = A * (HALF_STEP[t] * 1.01 + 2 * ds + (seen + 64) * 2.0 ** -23) + 2.0 ** -31 * np.abs(V).sum(0) * (t == "f16") + np.abs(o[h]) * HALF_STEP[t] + TINY[t]
+                        e[h] = spread * HALF_STEP[t] * 1.01 + A * (2 * ds + (seen + 64) * 2.0 ** -23) + 2.0 ** -31 * np.abs(V).sum(0) * (t == "f16") + np.abs(o[h]) * HALF_STEP[t] + TINY[t]
             out[q_start[b] + i] = (o, e)
     return out
 

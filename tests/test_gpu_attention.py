@@ -324,3 +324,24 @@ def test_shares_of_lengths_that_lead_out_of_the_buffers(dim):
     c.run()
     c.free()
     one(42, [4, 4], [20, 20], (4, 2), 64, "f16")
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("below", [3, 12, 18, 22, 26])
+@pytest.mark.parametrize("nq", [1, 40])
+def test_many_small_weights_beside_a_large_one(nq, below, t):
+    """One key of weight 1 and value 0, thousands of weight 2^-below and value 1: small weights count in both sums alike."""
+    def edit(c, q, k, v):
+        q[:], k[:], v[:] = 0.0, 0.0, 1.0
+        q[:, :, 0], k[5, :, 0], v[5] = 1.0, below, 0.0
+
+    one(43, [nq], [9000], (4, 1), 64, t, edit=edit, scale=float(np.log(2.0)))
+
+
+def test_a_row_of_one_key_is_its_value():
+    c = Call(44, [1, 1, 1, 70], [1, 1, 1, 70], (4, 2), 128, "bf16", packed=True).run()
+    v = op.narrow(c.v, "bf16")[0].reshape(c.rows, 2, 128)
+    for row in range(4):  # (the fourth is the first query of the last sequence)
+        got = c.got[row].reshape(4, 128)
+        assert all((got[h].view(np.uint16) == v[row, h // 2].view(np.uint16)).all() for h in range(4)), row
+    c.free()
