@@ -467,11 +467,12 @@ template <int T> __device__ __forceinline__ void write4(const AttnParams &p, con
 }
 
 // ------------------------------------------------------------------------------------------------ TILE: rows over wavefronts
-// Bound by the matrix units' feed and the power it draws: one prompt of 8192 tokens, 20 heads of 128 on 5, bf16: 344 GFLOP in 325 to 345 us, 1.0 to 1.06 PFLOP/s, where a
-// product of two 8192 x 8192 matrices reaches 1.21 on the same card.  64 KB of LDS leave two workgroups to a compute unit, and
+// Bound by the matrix units' feed: one prompt of 8192 tokens, 20 heads of 128 on 5, bf16: 344 GFLOP in 330 to 345 us, 1.0 PFLOP/s, where
+// a product of two 8192 x 8192 matrices reaches 1.21 on the same card; matrix units busy 56 % of the cycles, at 1.7 to 1.8 GHz.  64 KB of LDS leave two workgroups to a compute unit, and
 // one's exponentials run beside the other's products; of the time, the exponentials alone are a tenth, the loads 3 %.  Four
 // wavefronts of 32 rows share each tile of K and V through the LDS (without bank conflicts); of 256 rows: slower, one workgroup a unit.
-// Keys begin .. end - 1 (begin a multiple of the tile of keys, end one too or the last key that a row sees) for the 128 rows of t.
+//
+// Keys begin .. end - 1 (begin a multiple of the tile of keys, end one too or the last key that a row sees) for the 32 * WAVES rows of t.
 // part < 0: the rows are done and written; else their sums become part `part` in the workspace.
 template <int T, int DP, int KT, int WAVES> __device__ __forceinline__ void tile_rows(const AttnParams &p, const Tile &t, int kv_head, int begin, int end, int i_last, char *k_a, char *k_b,
                                                                                       char *v_a, char *v_b, int part)
@@ -541,7 +542,7 @@ template <int T, int DP, int KT, int WAVES> __device__ __forceinline__ void tile
     if (part >= 0 && lane < 32) p.part_ml[part_row] = float2{r.top, sum};
 }
 
-// SHARED: the blocks of keys of all tiles, tile after tile, are cut into equal shares, one a workgroup; a share may end within a tile
+// SHARED (four chunks of 130 to 250 tokens against 12000 to 20000 keys, 134 GFLOP: 160 us, and 17 for the join): the blocks of keys of all tiles, tile after tile, are cut into equal shares, one a workgroup; a share may end within a tile
 // and go on in the next.  A tile that lies in one share is written; others leave their sums, a workgroup at most two: of a
 // tile that it ends (part 0) and of one that it begins (part 1).  Neighbouring shares, which read the same keys, go to one XCD.
 template <int T, int DP, int KT, int WAVES, bool SHARED> __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) attention_tile_kernel(const AttnParams p)
