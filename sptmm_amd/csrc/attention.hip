@@ -542,9 +542,10 @@ template <int T, int DP, int KT, int WAVES> __device__ __forceinline__ void tile
     if (part >= 0 && lane < 32) p.part_ml[part_row] = float2{r.top, sum};
 }
 
-// SHARED (four chunks of 130 to 250 tokens against 12000 to 20000 keys, 134 GFLOP: 160 us, and 17 for the join): the blocks of keys of all tiles, tile after tile, are cut into equal shares, one a workgroup; a share may end within a tile
+// SHARED: the blocks of keys of all tiles, tile after tile, are cut into equal shares, one a workgroup; a share may end within a tile
 // and go on in the next.  A tile that lies in one share is written; others leave their sums, a workgroup at most two: of a
 // tile that it ends (part 0) and of one that it begins (part 1).  Neighbouring shares, which read the same keys, go to one XCD.
+// Four chunks of 130 to 250 tokens against 12000 to 20000 keys, 134 GFLOP: 160 us, and 17 for the join.
 template <int T, int DP, int KT, int WAVES, bool SHARED> __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) attention_tile_kernel(const AttnParams p)
 {
     __shared__ __attribute__((aligned(1024))) char k_a[KT * DP * 2], k_b[KT * DP * 2], v_a[KT * DP * 2], v_b[KT * DP * 2];

@@ -345,3 +345,12 @@ def test_a_row_of_one_key_is_its_value():
         got = c.got[row].reshape(4, 128)
         assert all((got[h].view(np.uint16) == v[row, h // 2].view(np.uint16)).all() for h in range(4)), row
     c.free()
+
+
+@pytest.mark.parametrize("nq", [[1, 1], [40, 3]])
+def test_no_cache_at_all(nq):
+    """kv_rows 0, k and v NULL: every row sees nothing and becomes zeros."""
+    c = Call(45, nq, [0, 0], (20, 5), 64, "f16", tail=1)
+    c.args.k = c.args.v = None
+    c.args.kv_rows = 0
+    c.run().check().free()
