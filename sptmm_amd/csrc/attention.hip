@@ -634,14 +634,15 @@ template <int T, int DP, int WAVES, bool STREAM> __global__ void __launch_bounds
         load(i + 1, k_a, v_a);
         r.template step<R::EDGE>(p, kb, vb, j, lo, r.polluted(vb, j, end, lo));
     }
-    // the wavefronts' sums, brought to one maximum and added in wavefront order; a wavefront's part lies where its tiles lay
+    // the wavefronts' sums, brought to one maximum and added in wavefront order; a wavefront's part lies where its tiles lay.  Where a
+    // wavefront has no maximum its sums are zeros, or NaN (the maximum passes over scores that are NaN), and are added as they are.
     const float sum = halves_sum(r.sum);
     if (lane < 32) tops[wave][lane] = r.top, sums[wave][lane] = sum;
     __syncthreads();
     float top = tops[0][lane & 31];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) top = fmaxf(top, tops[w][lane & 31]);
-    const float f = r.top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((r.top - top) * p.c);
+    const float f = r.top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((r.top - top) * p.c);
     constexpr int PER = ONE / 4096;  // blocks of 32 values of d that one array has room for
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -649,7 +650,7 @@ template <int T, int DP, int WAVES, bool STREAM> __global__ void __launch_bounds
         for (int e = 0; e < 4; ++e) {
             f32x4 x;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = r.top == -INFINITY ? 0.f : r.o[d][4 * e + i] * f;
+            for (int i = 0; i < 4; ++i) x[i] = r.o[d][4 * e + i] * f;
             *reinterpret_cast<f32x4 *>((d < PER ? k_a : v_a) + wave * ONE + (d % PER) * 4096 + e * 1024 + lane * 16) = x;
         }
     __syncthreads();
@@ -666,7 +667,7 @@ template <int T, int DP, int WAVES, bool STREAM> __global__ void __launch_bounds
         }
         float total = 0.f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) total += tops[w][rr] == -INFINITY ? 0.f : sums[w][rr] * __builtin_amdgcn_exp2f((tops[w][rr] - best) * p.c);
+        for (int w = 0; w < WAVES; ++w) total += sums[w][rr] * (tops[w][rr] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((tops[w][rr] - best) * p.c));
         const int row = t.row0 + rr, i = row / p.group;
         if (p.splits > 1) {
             const int64_t part_row = (int64_t)split * p.total_q * p.q_heads + (int64_t)(t.q0 + i) * p.q_heads + kv_head * p.group + row - i * p.group;

@@ -354,3 +354,16 @@ def test_no_cache_at_all(nq):
     c.args.k = c.args.v = None
     c.args.kv_rows = 0
     c.run().check().free()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("m", [1, 33, 64, 129, 161, 4000])
+def test_a_nan_in_a_key_that_a_row_sees_reaches_it_in_either_form(m, t):
+    """The last key alone, the last 32 of a tile, and everything from the middle on: keys of which a wavefront, or a split, may hold
+    nothing else.  max_q chooses the form; the other heads of the same token stay as they are."""
+    for first in sorted({m - 1, (m - 1) // 32 * 32, m // 2, 0}):
+        def edit(c, q, k, v):
+            k[first:m, 1, ::3] = np.nan
+
+        for max_q in (1, 200):
+            one(46, [1, 1], [m, 70], (20, 5), 128, t, edit=edit, max_q=max_q)
