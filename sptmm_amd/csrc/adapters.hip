@@ -5,7 +5,8 @@
 // In general two launches.  The first makes h: 16 rows of X against 16 ranks of A per matrix instruction (16-bit operands, 32-bit
 // sums), the rows' contraction over K split over wavefronts and workgroups.  The second adds up the splits' partial sums in
 // their order and multiplies by B on the 32-bit matrix instruction: h is never rounded to 16 bits -- outputs are 32-bit
-// floats, and a rounded h would cost them fifteen of their bits -- and B's 16-bit values are exact in 32.
+// floats, and a rounded h would cost them fifteen of their bits -- and B's 16-bit values are exact in 32.  (Many rows: on the 16-bit
+// instruction, by exact parts of both.)
 //
 // Rows come in any order of slots.  A tile of 16 rows is walked once per distinct slot in it (found by ballots, no sorting
 // pass); a matrix column is a row of X and stays in its lanes throughout, so rows of other slots are left out by a select
@@ -13,7 +14,7 @@
 //
 // Both weights sit in the order in which a wavefront reads them, 1 KiB per load instruction (adapters_pack_kernel).
 //
-// Many rows are bound by base, Y and X: 3001 rows, K=2560 N=13824, eight slots of rank 16 to 64: 356 MB in 101 us, 3.5 TB/s (an
+// Many rows are bound by base, Y and X: 3001 rows, K=2560 N=13824, eight slots of rank 16 to 64: 356 MB in 101 us (fp16 107), 3.5 TB/s (an
 // addition to an array of that size, 332 MB, 57 us).  A few rows are bound by latency: one row 6.7 to 8.3 us where an empty launch
 // takes 3.5; 48 rows of 32 slots, K=6912 N=2560: 18 MB in 13 to 15.5 us, two launches that each wait for slots, weights and sums.
 #include <atomic>
@@ -47,6 +48,7 @@ namespace sptmm {
 namespace {
 
 typedef unsigned short u16;
+typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
 typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
@@ -210,58 +212,51 @@ template <int T> __device__ __forceinline__ void add_chunk(u16x8 b, f32x4 h, boo
 #pragma unroll
     for (int e = 0; e < 4; ++e) y0[e] = mine ? n0[e] : y0[e], y1[e] = mine ? n1[e] : y1[e];
 }
-// The same on the 16-bit matrix instruction, an eighth (fp16) or a quarter (bf16) of its time: where many rows make the second product
-// long enough to stand beside its bytes.  A 32-bit h is the sum of parts of 16 bits, which share an instruction's 32 places along
-// the contraction with B's values given twice: three parts of bf16 are h exactly; of fp16, whose range is short, a row's h
-// is first brought below 2^15 by a power of two, and two parts hold 22 bits of it.  An h that is not finite is its first part; a
-// B that is not finite would meet the other parts' signs and zeros, and goes the 32-bit way.
+// The same on the 16-bit matrix instruction: where many rows make the second product long enough to stand beside its bytes.  A
+// 32-bit h is the sum of three parts of bf16, exactly and whatever its size (from 2^-102 on: no part is subnormal); a bf16 value of B is one part, an fp16 value (11 bits,
+// of the range of bf16) the sum of two.  Every part of B meets every part of h, two pairs of parts sharing an instruction's
+// 32 places along the contraction: two instructions to 16 columns (bf16) or three, each an eighth of the 32-bit way's time.  No bit of
+// the inner sums is lost: a small one beside a large one that the column does not use counts in full.  An h that is not
+// finite is its first part, and stays away from B's second one (infinity times that part's zeros is none of the product); a
+// B that is not finite goes the 32-bit way.
 template <int T> struct Parts {
-    float top = 0.f, scale = 1.f, back = 1.f;  // fp16: largest |h| of this lane's row, the power of two, and the way back
-    u16x8 first;
-    u16x8 third;
+    u16x8 h12, h31, h23;  // parts of h, by the pairs that an instruction takes (bf16: the first two; the upper half of h31 is zero)
 
-    __device__ __forceinline__ void add(f32x4 h)
-    {
-        if constexpr (T == SPTMM_X_F16)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = fabsf(h[e]) < INFINITY ? fmaxf(top, fabsf(h[e])) : top;
-    }
-    __device__ __forceinline__ void settle()
-    {
-        if constexpr (T == SPTMM_X_F16) {  // (a row's four lanes)
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const int e = max((int)(__builtin_bit_cast(unsigned, top) >> 23), 27) - 127 - 14;  // top < 2^(e + 15)
-            scale = __builtin_bit_cast(float, (unsigned)(127 - e) << 23);
-            back = __builtin_bit_cast(float, (unsigned)(127 + e) << 23);
-        }
-    }
+    static __device__ __forceinline__ unsigned top_bits(float x) { return __builtin_bit_cast(unsigned, x) & 0xffff0000u; }
     __device__ __forceinline__ void split(f32x4 h)
     {
-        third = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float x = h[e];
-            if constexpr (T == SPTMM_X_F16) {
-                const float y = x * scale;
-                const _Float16 hi = (_Float16)y;
-                const _Float16 lo = fabsf(y) < INFINITY ? (_Float16)(y - (float)hi) : (_Float16)0.f;
-                first[e] = __builtin_bit_cast(u16, hi), first[4 + e] = __builtin_bit_cast(u16, lo);
-            } else {
-                const bool finite = fabsf(x) < INFINITY;
-                const unsigned hi = __builtin_bit_cast(unsigned, x) & 0xffff0000u;
-                const float r = finite ? x - __builtin_bit_cast(float, hi) : 0.f;
-                const unsigned mid = __builtin_bit_cast(unsigned, r) & 0xffff0000u;
-                const float rest = r - __builtin_bit_cast(float, mid);
-                first[e] = (u16)(hi >> 16), first[4 + e] = (u16)(mid >> 16), third[e] = (u16)(__builtin_bit_cast(unsigned, rest) >> 16);
+            const bool finite = fabsf(x) < INFINITY;
+            const unsigned hi = top_bits(x);
+            const float r = finite ? x - __builtin_bit_cast(float, hi) : 0.f;
+            const unsigned mid = top_bits(r);
+            const u16 one = (u16)(hi >> 16), two = (u16)(mid >> 16), three = (u16)(top_bits(r - __builtin_bit_cast(float, mid)) >> 16);
+            h12[e] = one, h12[4 + e] = two, h31[e] = three, h31[4 + e] = T == SPTMM_X_F16 && finite ? one : (u16)0;
+            if constexpr (T == SPTMM_X_F16) h23[e] = two, h23[4 + e] = three;
+        }
+    }
+    // 16 columns: x holds four ranks' values of B
+    __device__ __forceinline__ f32x4 columns(u16x4 x, f32x4 y) const
+    {
+        if constexpr (T == SPTMM_X_F16) {
+            u16x8 b;  // its two parts
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v = widen<T>(x[e]);
+                const unsigned hi = top_bits(v);
+                b[e] = (u16)(hi >> 16), b[4 + e] = (u16)(__builtin_bit_cast(unsigned, v - __builtin_bit_cast(float, hi)) >> 16);
             }
+            return mfma16<SPTMM_X_BF16>(b, h31, mfma16<SPTMM_X_BF16>(b, h23, mfma16<SPTMM_X_BF16>(b, h12, y)));
+        } else {
+            const u16x8 b = __builtin_shufflevector(x, x, 0, 1, 2, 3, 0, 1, 2, 3);
+            return mfma16<T>(b, h31, mfma16<T>(b, h12, y));
         }
     }
     __device__ __forceinline__ void add_chunk(u16x8 b, bool mine, f32x4 &y0, f32x4 &y1) const
     {
-        const u16x8 b0 = __builtin_shufflevector(b, b, 0, 1, 2, 3, 0, 1, 2, 3), b1 = __builtin_shufflevector(b, b, 4, 5, 6, 7, 4, 5, 6, 7);
-        f32x4 n0 = mfma16<T>(b0, first, y0), n1 = mfma16<T>(b1, first, y1);
-        if constexpr (T != SPTMM_X_F16) n0 = mfma16<T>(b0, third, n0), n1 = mfma16<T>(b1, third, n1);
+        const f32x4 n0 = columns(__builtin_shufflevector(b, b, 0, 1, 2, 3), y0), n1 = columns(__builtin_shufflevector(b, b, 4, 5, 6, 7), y1);
 #pragma unroll
         for (int e = 0; e < 4; ++e) y0[e] = mine ? n0[e] : y0[e], y1[e] = mine ? n1[e] : y1[e];
     }
@@ -336,7 +331,6 @@ template <int T, int CP, bool ROWS> __global__ void __launch_bounds__(256) adapt
     const SlotInfo mine = slot >= 0 && write ? p.info[slot] : SlotInfo{0, 0.f, 0, 0};
     const int my_chunks = chunks_of(mine.rank);
     const unsigned long long wide = __ballot(mine.rank && mine.bad == mine.set);  // rows whose B takes the 32-bit instruction
-    Parts<T> big;
     f32x4 *const h_tile = h_lds + (ROWS ? wave * p.max_chunks * 64 : 0);
     for (int c = ROWS ? 0 : wave; c < p.max_chunks; c += ROWS ? 1 : 4) {
         if (!__ballot(c < my_chunks)) break;
@@ -352,34 +346,26 @@ template <int T, int CP, bool ROWS> __global__ void __launch_bounds__(256) adapt
             for (; k < p.splits; ++k) h += hp[k * next];
             h *= mine.scale;
             h_tile[c * 64 + lane] = h;
-            if constexpr (ROWS) big.add(h);
         }
     }
     __syncthreads();
     if (cols <= 0) return;
-    if constexpr (ROWS) big.settle();
-    // (fp16 parts are scaled: their sums stand apart until the end)
-    constexpr bool APART = ROWS && T == SPTMM_X_F16;
-    f32x4 sum[CP][2];
-    if constexpr (APART)
-#pragma unroll
-        for (int c = 0; c < CP; ++c) sum[c][0] = sum[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Parts<T> parts;
     while (now.s >= 0) {
         const Place then = after(now);
         u16x8 next[DEEP][CP];
         load(then, next);
-        const bool serves = slot == now.s, parts = ROWS && !(wide & __ballot(serves));
+        const bool serves = slot == now.s, by_parts = ROWS && !(wide & __ballot(serves));
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {
             if (now.c + d >= now.chunks) break;
             const f32x4 h = h_tile[(now.c + d) * 64 + lane];
-            if (parts) big.split(h);
+            if (by_parts) parts.split(h);
 #pragma unroll
             for (int i = 0; i < CP; ++i)
                 if (2 * i < cols) {
-                    if (!parts) add_chunk<T>(b[d][i], h, serves, acc[i][0], acc[i][1]);
-                    else if constexpr (APART) big.add_chunk(b[d][i], serves, sum[i][0], sum[i][1]);
-                    else big.add_chunk(b[d][i], serves, acc[i][0], acc[i][1]);
+                    if (by_parts) parts.add_chunk(b[d][i], serves, acc[i][0], acc[i][1]);
+                    else add_chunk<T>(b[d][i], h, serves, acc[i][0], acc[i][1]);
                 }
         }
 #pragma unroll
@@ -391,12 +377,8 @@ template <int T, int CP, bool ROWS> __global__ void __launch_bounds__(256) adapt
 #pragma unroll
     for (int c = 0; c < CP; ++c)
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            if constexpr (APART)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[c][g][e] = fmaf(sum[c][g][e], big.back, acc[c][g][e]);
+        for (int g = 0; g < 2; ++g)
             if (write && 2 * c + g < cols) *reinterpret_cast<f32x4 *>(p.Y + at + 32 * c + 16 * g) = acc[c][g];
-        }
 }
 
 // ------------------------------------------------------------------------------------------------ both products in one launch
@@ -491,8 +473,11 @@ template <int T> void launch_apply(const AdapterArgs &p, bool one_launch, hipStr
     hipLaunchKernelGGL((adapters_shrink_kernel<T>), dim3(p.tiles, p.splits, z), dim3(SHRINK_WAVES * 64), 0, st, p);
     // Fewer workgroups of the many-row kind than this leave compute units idle.  K=2560, ranks 8 to 64 of 32 slots, rows in any order
     // (in prompts), without and with it: 512 x 3840 (240 workgroups) 63, 65 us (16.8, 20.6); 1024 x 2560 (320) 78, 81 (18.9, 21.8);
-    // 512 x 6912 (432) 85, 72 (21.8, 22.7); 1024 x 6912 (864) 140, 105 (30.5, 26.6); 3001 x 13824 in prompts 127, 102.
-    if ((int64_t)(p.tiles / 4) * groups < 400)
+    // 512 x 6912 (432) 85, 72 (21.8, 22.7); 1024 x 6912 (864) 140, 105 (30.5, 26.6); 3001 x 13824 in prompts 127, 102.  fp16, whose B
+    // comes apart on the way: 512 x 6912 83, 86 (23.3, 24.9); 1024 x 6912 140, 129 (34.9, 31.6); 1024 x 13824 243, 194 (60.5, 53.6);
+    // 3001 x 13824 in prompts of rank 16 to 64 142, 107, of 64 to 128 196, 161, of 96 to 192 235, 222, and of 128 to 256 288, 349: there
+    // the sums of four tiles fill the LDS.
+    if ((int64_t)(p.tiles / 4) * groups < 400 || (T == SPTMM_X_F16 && p.max_chunks > 12))
         hipLaunchKernelGGL((adapters_expand_kernel<T, 1, false>), dim3(p.tiles * groups, 1, p.places), dim3(256), lds, st, p);
     else
         hipLaunchKernelGGL((adapters_expand_kernel<T, 4, true>), dim3((p.tiles + 3) / 4 * groups), dim3(256), 4 * lds, st, p);

@@ -249,3 +249,26 @@ def test_refusals():
     s.check(1, [0, 1, 0])
     for o in (X, S, Y, ws, s):
         o.free()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_a_small_inner_sum_beside_a_large_one_keeps_its_bits(t):
+    """Rank 0's inner sum is some 2^28 times rank 1's, and the even columns do not use it: what they add is rank 1's alone."""
+    s = Set(15, 48, 2064, t, [2, 3])
+
+    def edit(A, B):
+        A[0] *= 6e4
+        A[1] *= 2e-4
+        B[::2, 0] = 0.0
+
+    s.put(0, np.random.default_rng(1), 2, edit=edit)
+    for M in (5, 100, 2100):  # all three forms
+        s.check(2, np.arange(M) // 40 % 3 - 1, "none")
+    s.free()
+
+
+@pytest.mark.parametrize("rank", [192, 193, 256])
+def test_many_rows_of_large_ranks_in_fp16(rank):
+    s = Set(19, 32, 2064, "f16", [rank, 3, rank - 5], rank)
+    s.check(1, np.arange(2100) // 30 % 4 - 1)
+    s.free()
