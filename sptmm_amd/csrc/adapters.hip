@@ -17,19 +17,17 @@
 // Many rows are bound by base, Y and X: 3001 rows, K=2560 N=13824, eight slots of rank 16 to 64: 356 MB in 101 us (fp16 107), 3.5 TB/s (an
 // addition to an array of that size, 332 MB, 57 us).  A few rows are bound by latency: one row 6.7 to 8.3 us where an empty launch
 // takes 3.5; 48 rows of 32 slots, K=6912 N=2560: 18 MB in 13 to 15.5 us, two launches that each wait for slots, weights and sums.
-#include <atomic>
 #include <cmath>
 
 #include "internal.hpp"
 #include "lanes.hpp"
 
 namespace sptmm {
-// What the kernels know of a slot.  Its weights hold a value that is not finite where `bad` is the number of the call that set it
-// (found while packing, by many threads at once: they all write the same number, and none has to clear it first).
-struct SlotInfo {
+// What the kernels know of a slot.
+struct alignas(16) SlotInfo {
     int rank;  // 0: empty
     float scale;
-    int set, bad;
+    int bad;  // B holds a value that is not finite
 };
 }  // namespace sptmm
 
@@ -41,7 +39,6 @@ struct sptmm_adapters {
     int device, compute_units;
     uint16_t *A, *B;  // [slot]: [chunk][k_step][64 lanes][8] and [n_pair][chunk][64 lanes][8], packed by the chunks in use
     sptmm::SlotInfo *info;
-    std::atomic<int> sets{0};  // calls of sptmm_adapters_set so far
 };
 
 namespace sptmm {
@@ -77,13 +74,15 @@ struct AdapterArgs {
 };
 
 // ------------------------------------------------------------------------------------------------ weights into place
+// The slot's info, by a launch of its own before the weights': a captured set clears the mark anew with every replay.
+__global__ void adapters_info_kernel(SlotInfo *info, int rank, float scale) { *info = SlotInfo{rank, scale, 0}; }
+
 // One thread per stored value.  A lane of the first product's operand holds rank lane % 16, k = 8 * (lane / 16) + e of a step
 // of 32; of the second's, column lane % 16 (e < 4) or 16 + lane % 16 (e >= 4) of a pair, rank 4 * (lane / 16) + e % 4 of a chunk.
-__global__ void __launch_bounds__(256) adapters_pack_kernel(const u16 *A, const u16 *B, u16 *pA, u16 *pB, SlotInfo *info, int set, int rank, float scale, int K,
-                                                            int N, int k_steps, int n_pairs, int chunks, unsigned exponent)
+__global__ void __launch_bounds__(256) adapters_pack_kernel(const u16 *A, const u16 *B, u16 *pA, u16 *pB, SlotInfo *info, int rank, int K, int N, int k_steps, int n_pairs,
+                                                            int chunks, unsigned exponent)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i == 0) info->rank = rank, info->scale = scale, info->set = set;
     const int64_t na = (int64_t)chunks * k_steps * 512, nb = (int64_t)n_pairs * chunks * 512;
     const int e = (int)(i & 7), lane = (int)(i >> 3) & 63;
     if (i < na) {
@@ -97,7 +96,7 @@ __global__ void __launch_bounds__(256) adapters_pack_kernel(const u16 *A, const 
         const int n = 32 * pair + 16 * (e >> 2) + (lane & 15), r = 16 * c + 4 * (lane >> 4) + (e & 3);
         const u16 x = r < rank && n < N ? B[(int64_t)n * rank + r] : (u16)0;
         pB[i] = x;
-        if ((x & exponent) == exponent) info->bad = set;
+        if ((x & exponent) == exponent) info->bad = 1;
     }
 }
 
@@ -328,9 +327,9 @@ template <int T, int CP, bool ROWS> __global__ void __launch_bounds__(256) adapt
     u16x8 b[DEEP][CP];
     load(now, b);
 
-    const SlotInfo mine = slot >= 0 && write ? p.info[slot] : SlotInfo{0, 0.f, 0, 0};
+    const SlotInfo mine = slot >= 0 && write ? p.info[slot] : SlotInfo{0, 0.f, 0};
     const int my_chunks = chunks_of(mine.rank);
-    const unsigned long long wide = __ballot(mine.rank && mine.bad == mine.set);  // rows whose B takes the 32-bit instruction
+    const unsigned long long wide = __ballot(mine.rank && mine.bad);  // rows whose B takes the 32-bit instruction
     f32x4 *const h_tile = h_lds + (ROWS ? wave * p.max_chunks * 64 : 0);
     for (int c = ROWS ? 0 : wave; c < p.max_chunks; c += ROWS ? 1 : 4) {
         if (!__ballot(c < my_chunks)) break;
@@ -536,8 +535,10 @@ extern "C" int sptmm_adapters_set(sptmm_adapters *a, int slot, const uint16_t *A
     const int chunks = (rank + 15) / 16;
     const int64_t n = (int64_t)chunks * 512 * std::max(a->k_steps, a->n_pairs);
     u16 *pA = a->A + (size_t)slot * a->max_chunks * a->k_steps * 512, *pB = a->B + (size_t)slot * a->max_chunks * a->n_pairs * 512;
-    hipLaunchKernelGGL(adapters_pack_kernel, dim3((unsigned)std::max<int64_t>(1, (n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, A, B, pA, pB, a->info + slot,
-                       (a->sets++ & 0x3fffffff) + 1, rank, scale, a->K, a->N, a->k_steps, a->n_pairs, chunks, a->type == SPTMM_X_F16 ? 0x7c00u : 0x7f80u);
+    hipLaunchKernelGGL(adapters_info_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, a->info + slot, rank, scale);
+    if (n)
+        hipLaunchKernelGGL(adapters_pack_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, A, B, pA, pB, a->info + slot, rank, a->K, a->N, a->k_steps,
+                           a->n_pairs, chunks, a->type == SPTMM_X_F16 ? 0x7c00u : 0x7f80u);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? SPTMM_OK : hip_fail(e, "adapters_pack_kernel launch");
 }

@@ -272,3 +272,43 @@ def test_many_rows_of_large_ranks_in_fp16(rank):
     s = Set(19, 32, 2064, "f16", [rank, 3, rank - 5], rank)
     s.check(1, np.arange(2100) // 30 % 4 - 1)
     s.free()
+
+
+def test_a_captured_set_of_weights_is_what_its_buffers_hold():
+    """Replays of one captured set: with a B that is not finite, then with an ordinary one.  The second gives, bit for bit, what a
+    set that never held anything else gives."""
+    K, N, M, rank = 48, 2064, 2100, 16
+    st = sp.Stream()
+    r = np.random.default_rng(16)
+    (ab, a64), (bb, b64), (xb, x64) = (op.narrow(r.standard_normal(n), "bf16") for n in ((rank, K), (N, rank), (M, K)))
+    wild = bb.copy()
+    wild[70, 3] = 0x7F80  # infinity
+    A, B, X, S = (sp.DeviceBuffer.from_numpy(v) for v in (ab, wild, xb, np.zeros(M, np.int32)))
+    one, other = sp.Adapters(K, N, sp.X_BF16, 2, rank), sp.Adapters(K, N, sp.X_BF16, 2, rank)
+    n = one.workspace_bytes(M)
+    ws, Y, Z = sp.DeviceBuffer(n), sp.DeviceBuffer(4 * M * N), sp.DeviceBuffer(4 * M * N)
+    with sp.Graph(st) as g:
+        one.set(0, A, B, rank, 0.5, st)
+        one.apply(X, S, M, None, Y, ws, n, st)
+    for rep, b in enumerate((wild, bb, wild, bb)):
+        print("replay", rep, flush=True)
+        B.upload(b)
+        g.launch(st)
+        other.set(rep % 2, A, B, rank, 0.5, st)
+        S.upload(np.full(M, 0, np.int32))
+        st.sync()
+        got = Y.to_numpy(np.float32, (M, N))
+        with np.errstate(invalid="ignore"):
+            want, bound = op.adapters(x64, np.zeros(M, int), np.zeros((M, N)), [a64], [op.widen(b, "bf16")], [0.5])
+        fine = np.isfinite(want)
+        assert (np.isfinite(got) == fine).all() and (np.abs(got - want)[fine] <= bound[fine]).all()
+        fresh = sp.Adapters(K, N, sp.X_BF16, 2, rank)
+        fresh.set(0, A, B, rank, 0.5, st)
+        fresh.apply(X, S, M, None, Z, ws, n, st)
+        st.sync()
+        assert (Z.to_numpy(np.uint32, (M, N)) == got.view(np.uint32)).all(), rep
+        fresh.free()
+    g.destroy()
+    for o in (A, B, X, S, ws, Y, Z, one, other):
+        o.free()
+    st.destroy()
