@@ -419,7 +419,12 @@ template <int T> __global__ void __launch_bounds__(SHRINK_WAVES * 64) adapters_f
     if (write && second) *reinterpret_cast<f32x4 *>(p.Y + at + 16) = acc[1];
 }
 
-int hip_fail(hipError_t e, const char *what) { return fail(SPTMM_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e); }
+// (the runtime keeps a failed call's error until it is asked for: taken here, or the next launch would be blamed for it)
+int hip_fail(hipError_t e, const char *what)
+{
+    (void)hipGetLastError();
+    return e == hipErrorOutOfMemory ? fail(SPTMM_ERR_NOMEM, "%s: out of device memory", what) : fail(SPTMM_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
+}
 
 // One tile of rows, and A small (KiB of the largest slot, and of all workgroups' reads if every row has another slot): both
 // products run in one launch.  K=2560 N=3840, one row: rank 32 (160 KiB) 8.1 us, in two launches 11.2; rank 64 (320) 8.3 and 10.8;
@@ -518,7 +523,7 @@ extern "C" int sptmm_adapters_create(int K, int N, int type, int slots, int max_
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
         sptmm_adapters_free(a);
-        return e == hipErrorOutOfMemory ? fail(SPTMM_ERR_NOMEM, "out of device memory for %d adapters", slots) : hip_fail(e, "sptmm_adapters_create");
+        return hip_fail(e, "sptmm_adapters_create");
     }
     *out = a;
     return SPTMM_OK;

@@ -32,8 +32,10 @@ struct sptmm_weights {
 
 namespace {
 
+// (the runtime keeps a failed call's error until it is asked for: taken here, or the next launch would be blamed for it)
 int hip_fail(hipError_t e, const char *what)
 {
+    (void)hipGetLastError();
     return fail(SPTMM_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
 }
 #define HIP_TRY(expr)                                   \

@@ -312,3 +312,22 @@ def test_a_captured_set_of_weights_is_what_its_buffers_hold():
     for o in (A, B, X, S, ws, Y, Z, one, other):
         o.free()
     st.destroy()
+
+
+def test_a_refused_allocation_leaves_no_error_behind():
+    """35 TB of weights: refused.  The call after it, on the same thread, is not blamed for it."""
+    s = Set(17, 64, 64, "f16", [4, 2])
+    with pytest.raises(sp.SptmmError) as e:
+        sp.Adapters(1 << 20, 1 << 20, sp.X_F16, 65536, 256)
+    assert e.value.code == -4 and "memory" in str(e.value)
+    s.check(1, [0, 1, -1])
+    with pytest.raises(sp.SptmmError):
+        sp.DeviceBuffer(1 << 50)
+    X, slot, Y = sp.DeviceBuffer(2 * 64), sp.DeviceBuffer.from_numpy(np.zeros(1, np.int32)), sp.DeviceBuffer(4 * 64)
+    X.fill(0)
+    with pytest.raises(sp.SptmmError):
+        sp.DeviceBuffer(1 << 50)
+    s.a.apply(X, slot, 1, None, Y, None, 0)
+    sp.device_sync()
+    for o in (X, slot, Y, s):
+        o.free()
