@@ -97,22 +97,27 @@ def _stream(s):
 
 
 class _Args(C.Structure):
-    """Argument block built from keywords; device buffers as DeviceBuffer or address."""
+    """Argument block built from keywords; device buffers as DeviceBuffer (kept by the block while a field names it) or address."""
 
     def __init__(self, **fields):
         super().__init__()
+        object.__setattr__(self, "_held", {})  # field -> the object whose address the block holds
         for name, value in fields.items():
             setattr(self, name, value)
 
     def __setattr__(self, name, value):
         if name not in self._names:
             raise AttributeError("%s has no field %r" % (type(self).__name__, name))
+        held = None
         if isinstance(value, Rotation):
-            object.__setattr__(self, "_held", value)  # the block points at it
-            value = C.pointer(value)
+            held, value = value, C.pointer(value)
         elif isinstance(value, DeviceBuffer):
-            value = value.ptr
+            held, value = value, value.ptr
         super().__setattr__(name, value)
+        if held is not None:
+            self._held[name] = held
+        else:
+            self._held.pop(name, None)
 
 
 class HeadsArgs(_Args):

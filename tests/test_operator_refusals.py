@@ -90,3 +90,40 @@ def test_adapters_create_refuses(a):
     with pytest.raises(sp.SptmmError) as e:
         sp.Adapters(*a)
     assert e.value.code == -1
+
+
+def test_argument_blocks_keep_what_they_point_at():
+    """A block is kept from call to call: a buffer made for one of its fields must not be freed under it."""
+    import ctypes as C
+    import gc
+    import weakref
+
+    def buffer():
+        b = object.__new__(sp.DeviceBuffer)  # (no device needed: nothing allocated, nothing to free)
+        b.ptr, b.nbytes = C.c_void_p(), 0
+        return b, weakref.ref(b)
+
+    for args, field, other in ((heads_args(), "q_gain", "positions"), (attention_args(), "kv_len", "kv_start")):
+        b, seen = buffer()
+        setattr(args, field, b)
+        setattr(args, other, b)
+        del b
+        gc.collect()
+        assert seen() is not None
+        setattr(args, other, None)
+        gc.collect()
+        assert seen() is not None and getattr(args, other) is None
+        second, later = buffer()
+        setattr(args, field, second)
+        del second
+        gc.collect()
+        assert seen() is None and later() is not None  # replaced: the first is let go
+        setattr(args, field, 64)
+        gc.collect()
+        assert later() is None and getattr(args, field) == 64
+    a = heads_args(rotation=sp.Rotation([0.5, 0.25]))
+    a.tokens = 5
+    gc.collect()
+    assert a.rotation.contents.pairs == 2
+    a.rotation = None
+    assert not a.rotation
