@@ -340,8 +340,9 @@ int sptmm_gemv_batched(const sptmm_weights *const *ws, const void *const *X_dev,
  *   sptmm_adapters_apply: X [M][K] of the set's type (what sptmm_gemv_q8 takes), base and Y [M][N] float (what it leaves).
  *     base may be Y (added in place) or NULL (zeros).  row_slot[m] outside 0..slots-1, or an empty slot: Y[m] = base[m].
  *     Rows of one slot need not lie together.  An Inf or NaN in one row or one adapter reaches the rows that use it only.
- *     workspace_dev: sptmm_adapters_workspace_bytes(a, M) bytes (0: may be NULL), the caller's, reusable from call to call on one stream;
- *     calls that may overlap need one each.  X, base, Y and the workspace are aligned to 16 bytes.
+ *     workspace_dev: sptmm_adapters_workspace_bytes(a, M) bytes (0: may be NULL), enough for every call of up to M rows, the caller's,
+ *     reusable from call to call on one stream; calls that may overlap need one each.  X, base, Y and the workspace are aligned
+ *     to 16 bytes.
  * A set is used with the device current on which it was made (SPTMM_ERR_INVALID otherwise). */
 typedef struct sptmm_adapters sptmm_adapters; /* opaque; owns its device buffers */
 int sptmm_adapters_create(int K, int N, int type, int slots, int max_rank, sptmm_adapters **out);

@@ -457,6 +457,16 @@ size_t need(const sptmm_adapters *a, int M)
     return fused(a, M) ? 0 : (size_t)splits_of(a, M) * ((M + 15) / 16) * a->max_chunks * 64 * 16;
 }
 
+// The most that any call of up to M rows needs: fewer rows have more splits, and 4080 rows can need twice what 4096 do.  From as many
+// tiles as compute units on there is one split, and the need grows with the rows.
+size_t most_need(const sptmm_adapters *a, int M)
+{
+    size_t most = need(a, M);
+    for (int m = 1; m <= std::min(M, 128); ++m) most = std::max(most, need(a, m));
+    for (int m = 144; m <= M && m / 16 <= a->compute_units; m += 16) most = std::max(most, need(a, m));
+    return most;
+}
+
 int check_device(const sptmm_adapters *a)
 {
     int dev = -1;
@@ -551,7 +561,7 @@ extern "C" int sptmm_adapters_set(sptmm_adapters *a, int slot, const uint16_t *A
 extern "C" size_t sptmm_adapters_workspace_bytes(const sptmm_adapters *a, int M)
 {
     if (!a || M < 1) return 0;
-    return need(a, M);
+    return most_need(a, M);
 }
 
 extern "C" int sptmm_adapters_apply(const sptmm_adapters *a, const uint16_t *X, const int32_t *row_slot, int M, const float *base, float *Y, void *workspace,

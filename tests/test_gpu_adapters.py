@@ -331,3 +331,20 @@ def test_a_refused_allocation_leaves_no_error_behind():
     sp.device_sync()
     for o in (X, slot, Y, s):
         o.free()
+
+
+def test_one_workspace_for_the_largest_call_serves_the_smaller_ones():
+    s = Set(18, 2560, 64, "f16", [16, 3])
+    sizes = [4096, 4095, 4081, 4080, 2049, 1024, 1008, 500, 257, 130, 129, 128, 113, 112, 49, 48, 17, 16, 15, 2, 1]
+    n = s.a.workspace_bytes(4096)
+    assert all(s.a.workspace_bytes(a) >= s.a.workspace_bytes(b) for a, b in zip(sizes, sizes[1:]))
+    (xb, x64), slot = op.narrow(np.random.default_rng(1).standard_normal((4096, 2560)), "f16"), (np.arange(4096) % 3 - 1).astype(np.int32)
+    want, bound = op.adapters(x64, slot, np.zeros((4096, 64)), s.A, s.B, s.scale)
+    ws, X, Y, S = sp.DeviceBuffer(n), sp.DeviceBuffer.from_numpy(xb), sp.DeviceBuffer(4 * 4096 * 64), sp.DeviceBuffer.from_numpy(slot)
+    for M in sizes:
+        print("M", M, flush=True)
+        s.a.apply(X, S, M, None, Y, ws, n)
+        sp.device_sync()
+        assert (np.abs(Y.to_numpy(np.float32, (M, 64)) - want[:M]) <= bound[:M]).all()
+    for o in (ws, X, Y, S, s):
+        o.free()
