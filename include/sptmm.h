@@ -395,7 +395,9 @@ int sptmm_heads_norm_rotate(const sptmm_heads_args *args, void *stream);
  * max_q and max_kv (host side: at least the longest sequence's queries and keys) choose how the work is cut up; the results
  * are right whatever they say.
  * workspace_dev: sptmm_attention_workspace_bytes(args) bytes (0: may be NULL), aligned to 16, the caller's, reusable from
- * call to call on one stream; calls that may overlap need one each. */
+ * call to call on one stream; calls that may overlap need one each.  It is enough for the same call with any smaller max_kv.  A call
+ * of fewer sequences or rows may need more, as it is split further (64 sequences of one token: nothing; one of them alone:
+ * its parts): ask for each such size that will come, and take the largest. */
 typedef struct sptmm_attention_args {
     const uint16_t *q, *k, *v;
     uint16_t *out;

@@ -806,6 +806,7 @@ struct Cut {
     bool keys;  // the KEYS form
     bool stream;
     int dp, slots, splits, chunk, shares, log_rows;
+    int most_splits;  // of a call with these sizes and any max_kv up to this one
 };
 Cut cut(const sptmm_attention_args *a)
 {
@@ -819,14 +820,14 @@ Cut cut(const sptmm_attention_args *a)
     // workgroups of one tile each (those that have rows): about as many as sequences have tiles
     const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>(c.slots, c.keys ? (int64_t)a->batch : rows / tm + 1)) * a->kv_heads;
     const int max_kv = (int)std::min<int64_t>(a->max_kv, a->kv_rows);
-    c.splits = 1;
+    c.splits = c.most_splits = 1;
     if ((int64_t)a->total_q * a->q_heads >= (1 << 24)) {
         // (one launch of the join holds fewer rows)
     } else if (c.keys) {
         // Splits where these are fewer than the chip has places for, two per compute unit.
         const int unit = 128;  // keys a workgroup should have at least
         const int64_t want = (512 + tiles - 1) / tiles, most = (max_kv + unit - 1) / unit;
-        c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
+        c.splits = c.most_splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
         c.chunk = std::max(unit, (max_kv / c.splits + 127) / 128 * 128);
         c.splits = std::max(1, std::min(c.splits, (max_kv + c.chunk - 1) / c.chunk));
     } else {
@@ -893,7 +894,9 @@ using namespace sptmm;
 extern "C" size_t sptmm_attention_workspace_bytes(const sptmm_attention_args *a)
 {
     if (check(a) || a->batch == 0 || a->total_q == 0) return 0;
-    return workspace(a, cut(a));
+    Cut c = cut(a);
+    c.splits = c.most_splits;  // (a little longer cache can have fewer splits, of more keys each)
+    return workspace(a, c);
 }
 
 extern "C" int sptmm_attention(const sptmm_attention_args *a, void *workspace_dev, size_t workspace_bytes, void *stream)

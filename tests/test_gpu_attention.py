@@ -367,3 +367,19 @@ def test_a_nan_in_a_key_that_a_row_sees_reaches_it_in_either_form(m, t):
 
         for max_q in (1, 200):
             one(46, [1, 1], [m, 70], (20, 5), 128, t, edit=edit, max_q=max_q)
+
+
+def test_one_workspace_of_the_largest_need_serves_batches_of_every_size():
+    """64 sequences need no workspace and fewer do: the largest of all sizes' needs is asked for once and serves them all."""
+    calls = [Call(50 + n, [1] * n, [600 - 5 * i for i in range(n)], (16, 8), 64, "f16", max_kv=4000) for n in (64, 40, 9, 3, 1)]
+    needs = [sp.attention_workspace_bytes(c.args) for c in calls]
+    assert needs[0] == 0 and max(needs) > 0
+    ws = sp.DeviceBuffer(max(needs))
+    for c in calls:
+        print("batch", c.args.batch, flush=True)
+        c.ws = sp.DeviceBuffer(16)
+        sp.attention(c.args, ws, ws.nbytes)
+        sp.device_sync()
+        c.got = c.out.to_numpy(np.float16, c.before.shape)
+        c.check().free()
+    ws.free()

@@ -127,3 +127,11 @@ def test_argument_blocks_keep_what_they_point_at():
     assert a.rotation.contents.pairs == 2
     a.rotation = None
     assert not a.rotation
+
+
+@pytest.mark.parametrize("sizes", [dict(batch=1, total_q=1, max_q=1), dict(batch=7, total_q=7, max_q=1), dict(batch=3, total_q=20, max_q=8), dict(batch=2, total_q=150, max_q=100),
+                                   dict(batch=1, total_q=60, max_q=60, q_heads=40, kv_heads=8, q_stride=2560, out_stride=2560, k_stride=512, v_stride=512)])
+def test_a_workspace_for_the_longest_cache_serves_the_shorter_ones(sizes):
+    """max_kv grows from call to call while a cache fills: what the largest asks for is enough all the way."""
+    needs = [sp.attention_workspace_bytes(attention_args(max_kv=n, kv_rows=70000, **sizes)) for n in [*range(1, 3000, 7), *range(3000, 70000, 997)]]
+    assert needs[-1] > 0 and needs == sorted(needs)
