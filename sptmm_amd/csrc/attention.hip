@@ -829,7 +829,7 @@ Cut cut(const sptmm_attention_args *a)
         const int64_t want = (512 + tiles - 1) / tiles, most = (max_kv + unit - 1) / unit;
         c.splits = c.most_splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
         c.chunk = std::max(unit, (max_kv / c.splits + 127) / 128 * 128);
-        c.splits = std::max(1, std::min(c.splits, (max_kv + c.chunk - 1) / c.chunk));
+        c.splits = std::max(1, std::min(c.splits, (int)((max_kv + (int64_t)c.chunk - 1) / c.chunk)));
     } else {
         // Shares instead of a workgroup per tile where there are too few tiles to fill the chip evenly.  Heads of 128, bf16: four chunks
         // of 130 to 250 tokens against 12000 to 20000, 5 heads (140 tiles): shares 182 us, tiles 345; eight of 400 against 1400 to 20000
