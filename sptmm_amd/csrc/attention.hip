@@ -770,7 +770,8 @@ template <int T, int WAVES, bool SHARED> __global__ void __launch_bounds__(256) 
         blocks += w;
         if (!SHARED && c < 64) break;
     }
-    if (query >= s.q0 + s.nq) return;  // a row behind the last sequence
+    // a row behind the last sequence; or starts that are out of order, whose count names a sequence behind the row: no part is its own
+    if (query < s.q0 || query >= s.q0 + s.nq) return;
     u16 *const out = p.out + (int64_t)query * p.out_stride + (int64_t)head * p.dim;
     const int seen = s.nk - s.nq + (query - s.q0) + 1;
     if constexpr (SHARED) {

@@ -383,3 +383,42 @@ def test_one_workspace_of_the_largest_need_serves_batches_of_every_size():
         c.got = c.out.to_numpy(np.float16, c.before.shape)
         c.check().free()
     ws.free()
+
+
+@pytest.mark.parametrize("nq,max_q,heads,dim,max_kv", [([1, 1, 1, 1, 1], 1, (20, 5), 128, 3000), ([40, 9, 130, 2, 33], 200, (4, 2), 64, 100), ([40, 9, 130, 2, 33], 130, (6, 2), 128, 3000)])
+def test_arrays_that_lead_astray_write_nothing_beside_the_rows(nq, max_q, heads, dim, max_kv):
+    """All three forms, `out` between guard rows: cache rows and lengths of some sequences that lead out of the buffers (the others are
+    exact all the same), then starts of the queries that do (nothing beside `out` and the workspace is written)."""
+    c = Call(60, nq, [900, 20, 2500, 300, 40], heads, dim, "f16", max_q=max_q, max_kv=max_kv, tail=3)
+    hq, guard = heads[0], 512
+    rows = np.full((c.total + 2 * guard, hq * dim), 0x5A5A, np.uint16)
+    rows[guard:-guard] = c.before.view(np.uint16)
+    big = sp.DeviceBuffer.from_numpy(rows)
+    c.args.out = big.ptr.value + 2 * guard * hq * dim
+    start, length = c.kv_start.copy(), c.kv_len.copy()
+    start[0], start[3] = -5, 1 << 30
+    length[0], length[2], length[3] = 1 << 30, -7, 1 << 30
+    n = sp.attention_workspace_bytes(c.args)
+    c.ws = sp.DeviceBuffer(n + 4096)
+
+    def call():
+        c.ws.fill(0xFF)
+        sp.attention(c.args, c.ws, n)
+        sp.device_sync()
+        got = big.to_numpy(np.uint16, rows.shape)
+        assert (got[:guard] == 0x5A5A).all() and (got[-guard:] == 0x5A5A).all()
+        assert (c.ws.to_numpy(np.uint8, n + 4096)[n:] == 0xFF).all()
+        return got[guard:-guard]
+
+    c.bufs[4].upload(start), c.bufs[5].upload(length)
+    got = call()
+    assert (got[-3:] == c.before[-3:].view(np.uint16)).all()  # the rows behind the last sequence
+    values = op.widen(got.view(np.float16), "f16")
+    want = op.attention(c.q, c.k, c.v, c.q_start, c.kv_start, np.array([0, c.kv_len[1], 0, 0, c.kv_len[4]]), c.scale, "f16")
+    for row in [*range(c.q_start[1], c.q_start[2]), *range(c.q_start[4], c.q_start[5])]:
+        assert (np.abs(values[row].reshape(hq, dim) - want[row][0]) <= want[row][1]).all(), row
+    for bad in ([0, 9, 3, 1 << 30, 5, 7], [0, 60, 1, 70, 2, c.total], [-(1 << 31), (1 << 31) - 1] * 3, [(1 << 31) - 1, -1, 0, 1 << 30, 2, c.total + 1], [c.total] * 3 + [0, c.total, 1 << 30]):
+        c.bufs[3].upload(np.array(bad, np.int64).astype(np.int32))
+        call()
+    big.free()
+    c.free()
