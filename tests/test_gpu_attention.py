@@ -422,3 +422,35 @@ def test_arrays_that_lead_astray_write_nothing_beside_the_rows(nq, max_q, heads,
         call()
     big.free()
     c.free()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("nq,nk,max_q,max_kv", [([1, 1, 1], [300, 0, 77], 1, 2000), ([5, 70, 2], [5, 70, 2], 70, 70), ([30, 40, 9], [30, 1400, 600], 60, 2000)])
+def test_rows_before_the_first_sequence_and_strides_of_their_own(nq, nk, max_q, max_kv, packed):
+    """Starts that do not begin at 0, every buffer with another row stride, out's a multiple of 4 only."""
+    hq, hkv, dim, before = 6, 2, 64, 11
+    nk = nq if packed else nk
+    r = np.random.default_rng(70)
+    first = (before + np.concatenate([[0], np.cumsum(nq)])).astype(np.int32)
+    start = first[:-1].copy() if packed else (3 + np.concatenate([[0], np.cumsum(nk)[:-1]])).astype(np.int32)
+    total, rows = int(first[-1]) + 2, int(max(start + nk)) + 1
+    (q, q64), (k, k64), (v, v64), (out, _) = (op.narrow(r.standard_normal((n, h * dim + pad)), "bf16") for n, h, pad in ((total, hq, 8), (rows, hkv, 40), (rows, hkv, 0), (total, hq, 4)))
+    bufs = [sp.DeviceBuffer.from_numpy(x) for x in (q, k, v, out, first, start, np.asarray(nk, np.int32))]
+    a = sp.AttentionArgs(q=bufs[0], k=bufs[1], v=bufs[2], out=bufs[3], q_stride=hq * dim + 8, k_stride=hkv * dim + 40, v_stride=hkv * dim, out_stride=hq * dim + 4, kv_rows=rows, q_start=bufs[4],
+                         kv_start=None if packed else bufs[5], kv_len=None if packed else bufs[6], batch=len(nq), total_q=total, max_q=max_q, max_kv=max_kv, q_heads=hq, kv_heads=hkv, head_dim=dim,
+                         type=sp.X_BF16, scale=op.softmax_scale(dim))
+    ws = sp.DeviceBuffer(sp.attention_workspace_bytes(a) + 16)
+    ws.fill(0xFF)
+    print("rows before", nq, nk, packed, flush=True)
+    sp.attention(a, ws, ws.nbytes)
+    sp.device_sync()
+    got = bufs[3].to_numpy(np.uint16, out.shape)
+    want = op.attention(q64[:, : hq * dim].reshape(total, hq, dim), k64[:, : hkv * dim].reshape(rows, hkv, dim), v64.reshape(rows, hkv, dim), first, start, nk, a.scale, "bf16")
+    for row in range(total):
+        if row not in want:
+            assert (got[row] == out[row]).all(), row
+            continue
+        assert (got[row, hq * dim:] == out[row, hq * dim:]).all()
+        assert (np.abs(op.widen(got[row, : hq * dim], "bf16").reshape(hq, dim) - want[row][0]) <= want[row][1]).all(), row
+    for b in [ws] + bufs:
+        b.free()
