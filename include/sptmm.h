@@ -354,8 +354,9 @@ void sptmm_adapters_free(sptmm_adapters *a);
 
 /* Angles of a rotation by position: pair j of a head turns by position * radians_per_position[j] (for the usual geometric
  * sequence base^(-2j / rotated)).  interleaved 0: pair j is elements j and j + pairs; 1: elements 2j and 2j + 1.  Elements from
- * 2 * pairs on are not turned.  The frequencies are kept as 64-bit fractions of a turn, so the phase of any 32-bit
- * position is exact to 2^-33 of a turn.  Plain data: copy it, keep it on the stack. */
+ * 2 * pairs on are not turned.  The frequencies are kept as 64-bit fractions of a turn, and the phase of any 32-bit position is
+ * cut to 2^-32 of a turn; its distance from the nearest quarter turn is then rounded to a float, by 2^-28 of a turn at most.
+ * Plain data: copy it, keep it on the stack. */
 #define SPTMM_MAX_ROTATED_PAIRS 128
 typedef struct sptmm_rotation {
     int pairs;
@@ -389,7 +390,10 @@ int sptmm_heads_norm_rotate(const sptmm_heads_args *args, void *stream);
  * and the keys and values kv_start[b] .. kv_start[b]+kv_len[b]-1 of the cache; its query i of n sees keys j <= kv_len[b] - n + i
  * (whole prompts: n = kv_len; one token against a cache: n = 1; chunks of prompts in between; rows that see nothing become
  * zeros).  kv_start and kv_len NULL: the keys are packed as the queries are (k and v have at
- * least q_start[batch] rows).  Query head h reads key/value head h / (q_heads / kv_heads).  `out` overlaps no input.  16-bit inputs and outputs; products summed, and softmax statistics kept, in 32 bits.
+ * least q_start[batch] rows).  Query head h reads key/value head h / (q_heads / kv_heads).  `out` overlaps no input.  16-bit inputs and outputs; products
+ * summed, and softmax statistics kept, in 32 bits.  The weights exp(score - maximum) are rounded to the inputs' type for the
+ * product with v and for the sum that divides it: an output is off by up to half a step (bf16 2^-8, fp16 2^-11) of the values' weighted
+ * mean distance from it, beside its own rounding, and fp16 weights below 2^-32 of the largest count as nothing.
  * Output row i depends on the keys and values it sees only: Inf or NaN in other rows of the cache do not reach it.  Rows of
  * `out` behind the last sequence are left as they were.
  * max_q and max_kv (host side: at least the longest sequence's queries and keys) choose how the work is cut up; the results

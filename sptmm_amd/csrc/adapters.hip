@@ -15,7 +15,7 @@
 // Both weights sit in the order in which a wavefront reads them, 1 KiB per load instruction (adapters_pack_kernel).
 //
 // Many rows are bound by base, Y and X: 3001 rows, K=2560 N=13824, eight slots of rank 16 to 64: 356 MB in 101 us (fp16 107), 3.5 TB/s (an
-// addition to an array of that size, 332 MB, 57 us).  A few rows are bound by latency: one row 6.7 to 8.3 us where an empty launch
+// addition to an array of that size, 332 MB, 57 us).  A few rows are bound by latency: one row 6.7 to 8.6 us where an empty launch
 // takes 3.5; 48 rows of 32 slots, K=6912 N=2560: 18 MB in 13 to 15.5 us, two launches that each wait for slots, weights and sums.
 #include <cmath>
 
@@ -212,8 +212,8 @@ template <int T> __device__ __forceinline__ void add_chunk(u16x8 b, f32x4 h, boo
     for (int e = 0; e < 4; ++e) y0[e] = mine ? n0[e] : y0[e], y1[e] = mine ? n1[e] : y1[e];
 }
 // The same on the 16-bit matrix instruction: where many rows make the second product long enough to stand beside its bytes.  A
-// 32-bit h is the sum of three parts of bf16, exactly and whatever its size (from 2^-102 on: no part is subnormal); a bf16 value of B is one part, an fp16 value (11 bits,
-// of the range of bf16) the sum of two.  Every part of B meets every part of h, two pairs of parts sharing an instruction's
+// 32-bit h is the sum of three parts of bf16, exactly and whatever its size (from 2^-102 on: no part is subnormal); a bf16 value of B
+// is one part, an fp16 value (11 bits, of the range of bf16) the sum of two.  Every part of B meets every part of h, two pairs of parts sharing an instruction's
 // 32 places along the contraction: two instructions to 16 columns (bf16) or three, each an eighth of the 32-bit way's time.  No bit of
 // the inner sums is lost: a small one beside a large one that the column does not use counts in full.  An h that is not
 // finite is its first part, and stays away from B's second one (infinity times that part's zeros is none of the product); a

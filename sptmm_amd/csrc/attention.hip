@@ -467,8 +467,8 @@ template <int T> __device__ __forceinline__ void write4(const AttnParams &p, con
 }
 
 // ------------------------------------------------------------------------------------------------ TILE: rows over wavefronts
-// Bound by the matrix units' feed: one prompt of 8192 tokens, 20 heads of 128 on 5, bf16: 344 GFLOP in 330 to 345 us, 1.0 PFLOP/s, where
-// a product of two 8192 x 8192 matrices reaches 1.21 on the same card; matrix units busy 56 % of the cycles, at 1.7 to 1.8 GHz.  64 KB of LDS leave two workgroups to a compute unit, and
+// Bound by the matrix units' feed: one prompt of 8192 tokens, 20 heads of 128 on 5, bf16: 344 GFLOP in 315 to 347 us by card, 1.0 to 1.1 PFLOP/s, where
+// a product of two 8192 x 8192 matrices reaches 1.21; matrix units busy 54 % of the cycles, at 1.7 to 1.8 GHz.  64 KB of LDS leave two workgroups to a compute unit, and
 // one's exponentials run beside the other's products; of the time, the exponentials alone are a tenth, the loads 3 %.  Four
 // wavefronts of 32 rows share each tile of K and V through the LDS (without bank conflicts); of 256 rows: slower, one workgroup a unit.
 //
@@ -580,6 +580,8 @@ template <int T, int DP, int KT, int WAVES, bool SHARED> __global__ void __launc
 // Bound by the cache's read: 32 sequences of 2000 to 8000 keys, 661 MB, 5.5 TB/s.  Nothing is shared between wavefronts but the
 // sums at the end, so that each waits for its own loads only.  Two to a workgroup, as 128 KB of LDS for four leave one workgroup
 // to a compute unit: 20 heads of 128 on 5, one token against 8000 keys 13.7 us and 18.6, 32 against 1500 36 and 40, 64: 55 and 54.
+// Heads over 128 are far from this: the 32 offsets of a tile's loads do not fit the registers beside Q and O, every load waits for its
+// own from scratch memory, and 16 heads of 256 on 4, 32 caches of 0 to 16384 keys, 1059 MB, take 1950 us (0.54 TB/s).
 template <int T, int DP, int WAVES, bool STREAM> __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) attention_keys_kernel(const AttnParams p)
 {
     constexpr int KT = 32, LOG_TM = 5, ONE = KT * DP * 2;

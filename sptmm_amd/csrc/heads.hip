@@ -5,8 +5,8 @@
 //   (a, b) -> (a cos w - b sin w, b cos w + a sin w)      pair j of the first 2 * pairs elements, w = position * frequency_j
 //
 // The angle is kept as a fraction of a turn in 64-bit fixed point: turns_j = frequency_j / 2 pi as a fraction of 2^64, and
-// position * turns_j mod 2^64 is the phase, exact to position * 2^-65 turns however far the position -- no table of sines
-// to read, and no loss at far positions, where a product in 32 bits is off by position * 2^-24 radians.
+// position * turns_j mod 2^64 is the phase, right to position * 2^-65 turns however far the position, of which the upper 32 bits
+// are used -- no table of sines to read, and no loss at far positions, where a product in 32 bits is off by position * 2^-24 radians.
 // Everything is computed in 32 bits and rounded once, to nearest even, on the way out.
 //
 // The pass is bound by its bytes: 4096 tokens, 20 + 5 + 5 heads of 128, float in, bf16 out, 94 MB in 18.8 us (5.0 TB/s);
@@ -129,9 +129,9 @@ template <int OUT, bool INTER, bool WIDE> __device__ __forceinline__ void store8
     }
 }
 
-// Sine and cosine of the angle that position * turns / 2^64 is a fraction of a turn of.  The upper 32 bits of the phase are more
+// Sine and cosine of the angle that position * turns / 2^64 is a fraction of a turn of.  The phase is cut to its upper 32 bits, more
 // than a float holds; the nearest quarter turn is taken off them as an integer, and what is left, an eighth of a turn either
-// way, goes into the Taylor polynomials up to x^9 and x^8 (off by 2^-29 and 2^-25 at the ends).
+// way (rounded to 24 bits, by 2^-28 of a turn at most), goes into the Taylor polynomials up to x^9 and x^8 (off by 2^-29 and 2^-25 at the ends).
 __device__ __forceinline__ void turn(int position, unsigned turns_hi, unsigned turns_lo, float &sine, float &cosine)
 {
     const unsigned pos = (unsigned)position;
