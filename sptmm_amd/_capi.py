@@ -101,7 +101,6 @@ class _Args(C.Structure):
 
     def __init__(self, **fields):
         super().__init__()
-        object.__setattr__(self, "_held", {})  # field -> the object whose address the block holds
         for name, value in fields.items():
             setattr(self, name, value)
 
@@ -114,10 +113,11 @@ class _Args(C.Structure):
         elif isinstance(value, DeviceBuffer):
             held, value = value, value.ptr
         super().__setattr__(name, value)
+        kept = self.__dict__.setdefault("_held", {})  # field -> the object whose address the block holds (a copied block has none yet)
         if held is not None:
-            self._held[name] = held
+            kept[name] = held
         else:
-            self._held.pop(name, None)
+            kept.pop(name, None)
 
 
 class HeadsArgs(_Args):

@@ -135,3 +135,11 @@ def test_a_workspace_for_the_longest_cache_serves_the_shorter_ones(sizes):
     """max_kv grows from call to call while a cache fills: what the largest asks for is enough all the way."""
     needs = [sp.attention_workspace_bytes(attention_args(max_kv=n, kv_rows=70000, **sizes)) for n in [*range(1, 3000, 7), *range(3000, 70000, 997)]]
     assert needs[-1] > 0 and needs == sorted(needs)
+
+
+def test_copies_of_argument_blocks_can_be_changed():
+    a = attention_args()
+    for b in (sp.AttentionArgs.from_buffer_copy(a), sp.AttentionArgs()):
+        b.batch, b.q = 7, 8192
+        assert (b.batch, b.q) == (7, 8192)
+    assert a.batch == 2 and a.q == 4096
